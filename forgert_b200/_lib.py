@@ -20,10 +20,32 @@ FR_ERR_TIMEOUT = 5
 FR_ERR_WORKSPACE = 6
 FR_ERR_SCRATCH_LIMIT = 7
 
+FR_KV8_INT8 = 0
+FR_KV8_E4M3 = 1
+FR_KV8_BLOCK = 16
+
+FR_STEP_OK = 0
+FR_STEP_NO_PAGES = 1
+FR_STEP_BAD_LENGTH = 2
+FR_STEP_TOO_MANY = 3
+FR_STEP_BAD_FREE = 4
+
 # Every symbol include/forgert_attn.h declares, with its ctypes signature.
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _fp = ctypes.POINTER(ctypes.c_float)
+
+
+class Kv8CacheStruct(ctypes.Structure):
+    """fr_kv8_cache of include/forgert_attn.h."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("scales", _vp), ("dtype", _i), ("num_pages", _i),
+                ("page_size", _i), ("num_kv_heads", _i), ("head_dim", _i),
+                ("page_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong),
+                ("row_stride", ctypes.c_longlong)]
+
+
+_kv8 = ctypes.POINTER(Kv8CacheStruct)
 SIGNATURES = {
     "fr_decode_attn": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "fr_decode_attn_noalloc": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
@@ -60,6 +82,14 @@ SIGNATURES = {
     "fr_version": (_i, []),
     "fr_launch_count": (ctypes.c_ulonglong, []),
     "fr_set_launch_overlap": (_i, [_i]),
+    "fr_paged_step": (_i, [_vp] * 11 + [_i] * 5 + [_vp]),
+    "fr_qkv_rope_append_kv8": (_i, [_vp, _vp, _vp, _vp, _vp, _vp,
+                                    ctypes.POINTER(ctypes.c_longlong), _vp, _vp, _vp, _vp, _vp,
+                                    _i, _vp, _i, ctypes.c_char_p, _vp, _kv8, _i, _i, _vp]),
+    "fr_kv8_gather": (_i, [_kv8, _vp, _vp, _vp, _i, _vp]),
+    "fr_decode_attn_paged_kv8": (_i, [_vp, ctypes.c_longlong, _kv8, _vp, _vp, _vp, _i, _i, _i, _i,
+                                      _vp]),
+    "fr_kv8_workspace_size": (ctypes.c_size_t, [_i, _i, _i, _i, _i]),
     "fr_copy_async": (_i, [_vp, _vp, ctypes.c_size_t, _vp]),
 }
 

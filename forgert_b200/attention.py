@@ -13,6 +13,7 @@ from __future__ import annotations
 import ctypes
 from typing import Sequence
 
+from . import _lib
 from ._lib import ForgeRTError, check, load
 
 __all__ = [
@@ -21,6 +22,8 @@ __all__ = [
     "decode_attn_batched", "decode_attn_partial", "lse_merge", "rope_precompute_tables",
     "rope_tables_device",
     "rope_append", "reserve_workspace", "decode_workspace_size", "device_error",
+    "KV8Cache", "paged_step", "qkv_rope_append_kv8", "kv8_gather", "decode_attn_paged_kv8",
+    "kv8_workspace_size",
 ]
 
 
@@ -172,6 +175,117 @@ def qkv_bias_rope_append(q, k, v, q_bias, k_bias, v_bias, k_cache, v_cache, cos_
         _ptr(q), _ptr(k), _ptr(v), _ptr(q_bias), _ptr(k_bias), _ptr(v_bias), _ptr(k_cache),
         _ptr(v_cache), _ptr(cos_tab), _ptr(sin_tab), seq_len, num_heads, num_kv_heads, head_dim,
         pos_offset, _stream(stream)))
+
+
+class KV8Cache:
+    """A paged cache held in 8 bits (fr_kv8_cache): a value is code * scale.
+
+    k, v [num_pages, num_kv_heads, page_size, head_dim], torch.int8 or
+    torch.float8_e4m3fn, contiguous in the last dimension and both of the same
+    strides, else of any; scales [num_pages, num_kv_heads, page_size / 16, 2]
+    fp32, contiguous (a K and a V scale for each block of 16 rows and head).
+    The cache is the caller's memory: this keeps the tensors and their layout.
+    """
+
+    def __init__(self, k, v, scales):
+        import torch
+
+        codes = {torch.int8: _lib.FR_KV8_INT8, torch.float8_e4m3fn: _lib.FR_KV8_E4M3}
+        if k.dtype not in codes or v.dtype != k.dtype:
+            raise ValueError("k and v must both be torch.int8 or torch.float8_e4m3fn")
+        if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or k.stride(3) != 1:
+            raise ValueError("k and v must be [num_pages, num_kv_heads, page_size, head_dim] "
+                             "with equal strides, contiguous in the last dimension")
+        pages, heads, rows, dim = k.shape
+        if (scales.dtype != torch.float32 or not scales.is_contiguous() or
+                tuple(scales.shape) != (pages, heads, rows // _lib.FR_KV8_BLOCK, 2)):
+            raise ValueError("scales must be contiguous fp32 "
+                             "[num_pages, num_kv_heads, page_size / 16, 2]")
+        self.k, self.v, self.scales = k, v, scales
+        strides = [k.stride(i) for i in range(3)]
+        # a dimension of one element never steps: give it a stride the checks accept
+        strides = [s if n > 1 else max(s, -(-dim // 16) * 16) // 16 * 16
+                   for s, n in zip(strides, k.shape)]
+        self._struct = _lib.Kv8CacheStruct(
+            _ptr(k), _ptr(v), _ptr(scales), codes[k.dtype], pages, rows, heads, dim, *strides)
+        self._ref = ctypes.byref(self._struct)
+
+    @classmethod
+    def empty(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, dtype=None,
+              device="cuda"):
+        """A cache in fresh memory, page and head outermost."""
+        import torch
+
+        dtype = torch.int8 if dtype is None else dtype
+        k = torch.empty((num_pages, num_kv_heads, page_size, head_dim), dtype=dtype, device=device)
+        scales = torch.empty((num_pages, num_kv_heads, page_size // _lib.FR_KV8_BLOCK, 2),
+                             dtype=torch.float32, device=device)
+        return cls(k, torch.empty_like(k), scales)
+
+
+def paged_step(kv_lens, new_lens, block_table, free_pages, free_count, kv_lens_out,
+               free_count_out, token_offsets, positions, slots, status, batch: int,
+               page_size: int, num_pages: int, max_blocks_per_seq: int, max_tokens: int,
+               stream=None) -> None:
+    """Pages, positions and slots of one step's new tokens, on the GPU: kv_lens,
+    new_lens [batch] (a negative new length ends a request), block_table
+    [batch, max_blocks_per_seq] and the stack free_pages [num_pages] in place,
+    token_offsets [batch + 1], positions / slots (int64) [max_tokens].  status
+    [1] is FR_STEP_OK, or why the step was refused and nothing changed."""
+    lib = load()
+    check("fr_paged_step", lib.fr_paged_step(
+        _ptr(kv_lens), _ptr(new_lens), _ptr(block_table), _ptr(free_pages), _ptr(free_count),
+        _ptr(kv_lens_out), _ptr(free_count_out), _ptr(token_offsets), _ptr(positions),
+        _ptr(slots), _ptr(status), batch, page_size, num_pages, max_blocks_per_seq, max_tokens,
+        _stream(stream)))
+
+
+def qkv_rope_append_kv8(q, k, v, q_out, k_out, v_out, cos_tab, sin_tab, positions, slots,
+                        cache: KV8Cache, num_tokens: int, num_heads: int, table_rows: int,
+                        q_bias=None, k_bias=None, v_bias=None, num_axes: int = 1,
+                        freq_axis: bytes | None = None, token_strides=None, stream=None) -> None:
+    """Bias + RoPE on q/k and K/V coded into the 8-bit cache at `slots` (one
+    launch).  positions int32 [num_axes, num_tokens], freq_axis the axis of
+    each of the head_dim / 2 frequencies; k_out / v_out may be None (only the
+    cache is wanted) and every output its input; token_strides: halves between
+    tokens of q, k, v, q_out, k_out, v_out."""
+    lib = load()
+    if freq_axis is not None and len(freq_axis) != cache._struct.head_dim // 2:
+        raise ValueError("freq_axis must name an axis for each of the head_dim / 2 frequencies")
+    strides = None
+    if token_strides is not None:
+        strides = (ctypes.c_longlong * 6)(*token_strides)
+    check("fr_qkv_rope_append_kv8", lib.fr_qkv_rope_append_kv8(
+        _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(v_out), strides, _ptr(q_bias),
+        _ptr(k_bias), _ptr(v_bias), _ptr(cos_tab), _ptr(sin_tab), table_rows, _ptr(positions),
+        num_axes, freq_axis, _ptr(slots), cache._ref, num_tokens, num_heads, _stream(stream)))
+
+
+def kv8_gather(cache: KV8Cache, slots, k_out, v_out, num_slots: int, stream=None) -> None:
+    """Reads slots back as fp16 [num_slots, num_kv_heads, head_dim] (either
+    output may be None); a slot outside the pool gives zeros."""
+    lib = load()
+    check("fr_kv8_gather", lib.fr_kv8_gather(cache._ref, _ptr(slots), _ptr(k_out), _ptr(v_out),
+                                             num_slots, _stream(stream)))
+
+
+def decode_attn_paged_kv8(q, cache: KV8Cache, block_table, kv_lens, out, batch: int,
+                          num_heads: int, max_blocks_per_seq: int, max_kv_len: int,
+                          q_stride: int = 0, stream=None) -> None:
+    """Decode attention, one token per sequence, over the 8-bit paged cache:
+    q/out [batch, num_heads, head_dim] fp16 (q_stride halves between the
+    sequences' q, 0 = contiguous), block_table int32 [batch,
+    max_blocks_per_seq], kv_lens int32 [batch]."""
+    lib = load()
+    check("fr_decode_attn_paged_kv8", lib.fr_decode_attn_paged_kv8(
+        _ptr(q), q_stride, cache._ref, _ptr(block_table), _ptr(kv_lens), _ptr(out), batch,
+        num_heads, max_blocks_per_seq, max_kv_len, _stream(stream)))
+
+
+def kv8_workspace_size(batch: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                       max_kv_len: int) -> int:
+    return int(load().fr_kv8_workspace_size(batch, num_heads, num_kv_heads, head_dim,
+                                            max_kv_len))
 
 
 EXCHANGE_HEADER_BYTES = 256          # u32 epoch, u32 done

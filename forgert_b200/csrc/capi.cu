@@ -10,6 +10,9 @@
 #include "prefill_tc_kernels.cuh"
 #include "rope_kernels.cuh"
 #include "copy_kernels.cuh"
+#include "kv8_decode_kernels.cuh"
+#include "kv8_append_kernels.cuh"
+#include "paged_step_kernels.cuh"
 #include "../../include/forgert_attn.h"
 
 #include <cuda.h>
@@ -59,6 +62,8 @@ struct DeviceState {
     int persist_occ[4] = {0};    // CTAs/SM of the persistent batched kernels
     int resident[4][5] = {{-1, -1, -1, -1, -1}, {-1, -1, -1, -1, -1}, {-1, -1, -1, -1, -1},
                           {-1, -1, -1, -1, -1}};   // co-resident clusters per (slot, log2 size)
+    int kv8_occ[8] = {0};        // CTAs/SM of the 8-bit decode kernels (0 = not prepared)
+    bool step_ready = false;     // paged_step_kernel's shared-memory attribute set
     int resident_g[4][2] = {{-1, -1}, {-1, -1}, {-1, -1}, {-1, -1}};   // grouped form, 8 / 16
 };
 
@@ -1407,6 +1412,7 @@ int fr_get_device_error(int clear, int* device_code) {
         if (e != cudaSuccess) return cuda_fail(e);
     }
     if (device_code) *device_code = code;
+    if (code == fr::kDevBadIndex) return FR_ERR_INVALID_ARG;
     return code ? FR_ERR_TIMEOUT : FR_OK;
 }
 
@@ -1645,3 +1651,5 @@ extern "C" int fr_decode_attn_noalloc(const void* q, const void* k_cache, const 
                           : launch_merge<128>(p.part_ml, p.part_acc, pl.num_splits, ms, num_heads,
                                               o, nullptr, nullptr, 0, s);
 }
+
+#include "kv8_api.cuh"

@@ -21,6 +21,7 @@ enum DeviceError : int {
     kDevTimeoutFull = 1,   // consumer gave up waiting for a stage to land
     kDevTimeoutEmpty = 2,  // producer gave up waiting for a stage to drain
     kDevTimeoutPeer = 3,   // cross-GPU exchange: the other ranks' states never all arrived
+    kDevBadIndex = 4,      // a position or slot outside its table or pool (that token was not cached)
 };
 
 // Wall-clock budget of one bounded wait (ns).  Real waits last microseconds;
@@ -266,6 +267,33 @@ __device__ __forceinline__ void grid_dependency_wait() {
 
 __device__ __forceinline__ void grid_launch_dependents() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// ------------------------------------------------ small asynchronous copies
+// 8-byte copy into shared memory; src_bytes = 0 writes zeros and reads nothing.
+__device__ __forceinline__ void cp_async_8(uint32_t dst_smem, const void* src, uint32_t src_bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;"
+                 :: "r"(dst_smem), "l"(src), "r"(src_bytes) : "memory");
+}
+
+// Arrives on `bar` once this thread's earlier cp.async copies have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];"
+                 :: "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];"
+                 : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+    return v;
 }
 
 // ------------------------------------------------------------ tensor-core ops

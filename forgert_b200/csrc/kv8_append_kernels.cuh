@@ -1,0 +1,355 @@
+// kv8_append_kernels.cuh - decode/prefill prologue of the 8-bit paged cache:
+// q/k/v bias + RoPE (one or several position axes) + quantised append through
+// a slot map, in one launch; and the read-back of slots as fp16.
+//
+// Mathematics, per token t (all in fp32, one rounding at each output):
+//   x = x + bias;  for f < D/2 the pair (x[f], x[f + D/2]) of q and k turns to
+//   (a*c - b*s, a*s + b*c) with c, s = tables[positions[axis(f)][t]][f].
+// Append: consecutive tokens in consecutive rows of one block of 16 (a "run")
+// are coded together,
+//   scale = amax / kMax, at least the block's old scale if the run does not
+//   start the block;  code = round(x / scale), ties to even.
+// If that makes the scale grow, the block's earlier rows are coded anew:
+// code' = round(code * old / scale).  All runs of a block are the work of the
+// warp of its first token, in token order (more than one where a token between
+// them is left out), so the scale, the old rows and the new ones need no order
+// between warps.  The maximum is
+// taken over the bit patterns of |x|, where NaN is the largest: a block that
+// holds a NaN or an infinity gets such a scale and reads back as such.
+//
+// Layout: LPR = D / 8 lanes share a row, lane l holding the pairs f = 4l ..
+// 4l + 3: 8-byte loads of both halves, 4-byte code stores, a 16-byte load
+// each of cosines and sines.  A warp holds a whole 16-row run in registers
+// (every row's loads in flight at once) and so reads it once.
+#pragma once
+#include "fr_ptx.cuh"
+#include "decode_kernels.cuh"
+#include "kv8_common.cuh"
+#include <cstdint>
+
+namespace fr {
+
+constexpr int kAppendThreads = 128;
+constexpr int kMaxAxes = 4;
+constexpr int kQHeads = 4;              // query heads of a token that one lane group turns
+
+struct AppendParams {
+    const __half* q;
+    const __half* k;
+    const __half* v;
+    __half* q_out;
+    __half* k_out;                      // nullptr: not written
+    __half* v_out;
+    long long stride[6];                // halves between tokens: q, k, v, q_out, k_out, v_out
+    const __half* bias[3];
+    const float* cos_tab;
+    const float* sin_tab;
+    const int* positions;               // [axes][T]
+    const long long* slots;
+    Kv8View cache;
+    int* err;
+    int T, H, axes, table_rows;
+    uint8_t axis[64];                   // axis of frequency f
+};
+
+// Eight values of a row: its pairs 4l .. 4l + 3 (first halves, second halves).
+struct Row8 {
+    float lo[4], hi[4];
+};
+
+__device__ __forceinline__ void unpack4(uint2 w, float (&x)[4]) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+}
+
+__device__ __forceinline__ uint2 pack4(const float (&x)[4]) {
+    return make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+}
+
+template <int D>
+__device__ __forceinline__ Row8 load_row(const __half* row, int f0) {
+    Row8 r;
+    unpack4(*reinterpret_cast<const uint2*>(row + f0), r.lo);
+    unpack4(*reinterpret_cast<const uint2*>(row + f0 + D / 2), r.hi);
+    return r;
+}
+
+template <int D>
+__device__ __forceinline__ void store_row(__half* row, int f0, const Row8& r) {
+    *reinterpret_cast<uint2*>(row + f0) = pack4(r.lo);
+    *reinterpret_cast<uint2*>(row + f0 + D / 2) = pack4(r.hi);
+}
+
+// Cosines and sines of token t at the lane's four frequencies.  A position
+// outside the table is recorded and read as position 0.
+template <int D>
+__device__ __forceinline__ void load_turn(const AppendParams& p, int t, int f0, float (&c)[4],
+                                          float (&s)[4]) {
+    constexpr int kHalf = D / 2;
+    auto at = [&](int axis) {
+        int pos = p.positions[(size_t)axis * p.T + t];
+        if (pos < 0 || pos >= p.table_rows) {
+            record_error(p.err, kDevBadIndex);
+            pos = 0;
+        }
+        return pos;
+    };
+    if (p.axes == 1) {
+        const size_t e = (size_t)at(0) * kHalf + f0;
+        const float4 cv = *reinterpret_cast<const float4*>(p.cos_tab + e);
+        const float4 sv = *reinterpret_cast<const float4*>(p.sin_tab + e);
+        c[0] = cv.x; c[1] = cv.y; c[2] = cv.z; c[3] = cv.w;
+        s[0] = sv.x; s[1] = sv.y; s[2] = sv.z; s[3] = sv.w;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const size_t e = (size_t)at(p.axis[f0 + j]) * kHalf + f0 + j;
+        c[j] = p.cos_tab[e];
+        s[j] = p.sin_tab[e];
+    }
+}
+
+// The products are rounded before they are added, as separate operations
+// would: which codes a block gets does not hang on contraction.
+__device__ __forceinline__ void turn(Row8& r, const float (&c)[4], const float (&s)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float a = r.lo[j], b = r.hi[j];
+        r.lo[j] = __fsub_rn(__fmul_rn(a, c[j]), __fmul_rn(b, s[j]));
+        r.hi[j] = __fadd_rn(__fmul_rn(a, s[j]), __fmul_rn(b, c[j]));
+    }
+}
+
+__device__ __forceinline__ void add_bias(Row8& r, const Row8& b) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        r.lo[j] = __fadd_rn(r.lo[j], b.lo[j]);
+        r.hi[j] = __fadd_rn(r.hi[j], b.hi[j]);
+    }
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// x / scale to a code; scale 0 (a block of zeros) gives code 0.
+template <class Code>
+__device__ __forceinline__ uint32_t code4(const float (&x)[4], float scale) {
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = scale == 0.f ? 0.f : __fdiv_rn(x[j], scale);
+    return Code::encode4(y[0], y[1], y[2], y[3]);
+}
+
+// One run: rows t .. t + n - 1 (n <= 16) of K or V head h go to rows row0 ..
+// of the block at `slot`.  The whole warp takes part.
+template <int D, class Code>
+__device__ __forceinline__ void append_run(const AppendParams& p, int which, int h, int t, int n,
+                                           long long slot, const Row8& bias, bool biased,
+                                           int lane) {
+    constexpr int LPR = D / 8;
+    constexpr int RPW = 32 / LPR;               // rows per pass
+    constexpr int PASSES = kKv8Block / RPW;
+    const int sub = lane / LPR, f0 = (lane % LPR) * 4;
+    const Kv8View& c = p.cache;
+    const int page = int(slot / c.page_size), r0 = int(slot % c.page_size);
+    const int first = r0 % kKv8Block;           // rows of the block that are held already
+    const __half* x = (which ? p.v : p.k) + (size_t)h * D;
+    __half* y = which ? p.v_out : p.k_out;
+    const long long xs = p.stride[1 + which], ys = p.stride[4 + which];
+    uint8_t* pool = which ? c.v : c.k;
+    float* scale_at = reinterpret_cast<float*>(c.scale(page, h, r0)) + which;
+    const float old = first ? *scale_at : 0.f;
+
+    Row8 rows[PASSES];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int j = i * RPW + sub;
+        if (j < n) rows[i] = load_row<D>(x + (size_t)(t + j) * xs, f0);
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int j = i * RPW + sub;
+        if (j < n) {
+            if (biased) add_bias(rows[i], bias);
+            if (!which) {
+                float cc[4], ss[4];
+                load_turn<D>(p, t + j, f0, cc, ss);
+                turn(rows[i], cc, ss);
+            }
+            if (y) store_row<D>(y + (size_t)(t + j) * ys + (size_t)h * D, f0, rows[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                top = max(top, max(abs_bits(rows[i].lo[e]), abs_bits(rows[i].hi[e])));
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    float scale = __fdiv_rn(__uint_as_float(top), Code::kMax);
+    if (first) scale = __uint_as_float(max(abs_bits(scale), abs_bits(old)));
+    if (first && abs_bits(scale) > abs_bits(old)) {
+#pragma unroll 1
+        for (int j = sub; j < first; j += RPW) {
+            uint8_t* dst = pool + c.row(page, h, r0 - first + j);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t* w = reinterpret_cast<uint32_t*>(dst + f0 + e * (D / 2));
+                const uint32_t codes = *w;
+                float z[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) z[b] = __fmul_rn(Code::decode(codes >> (8 * b)), old);
+                *w = code4<Code>(z, scale);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int j = i * RPW + sub;
+        if (j < n) {
+            uint8_t* dst = pool + c.row(page, h, r0 + j);
+            *reinterpret_cast<uint32_t*>(dst + f0) = code4<Code>(rows[i].lo, scale);
+            *reinterpret_cast<uint32_t*>(dst + f0 + D / 2) = code4<Code>(rows[i].hi, scale);
+        }
+    }
+    if (lane == 0) *scale_at = scale;
+}
+
+// Warps 0 .. kv_tasks - 1: (WINDOW tokens, K or V, kv head), doing the blocks
+// that one of these tokens is the first of; the warps after them: query rows, a lane group per (token, kQHeads heads).
+template <int D, int WINDOW, class Code>
+__global__ void __launch_bounds__(kAppendThreads)
+kv8_append_kernel(const __grid_constant__ AppendParams p) {
+    constexpr int LPR = D / 8;
+    constexpr int RPW = 32 / LPR;
+    const int lane = threadIdx.x & 31;
+    const long long task = (long long)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
+    const int Hkv = p.cache.Hkv;
+    const int windows = (p.T + WINDOW - 1) / WINDOW;
+    const long long kv_tasks = 2LL * windows * Hkv;
+    const int f0 = (lane % LPR) * 4;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    if (task < kv_tasks) {
+        const int h = int(task % Hkv);
+        const int which = int(task / Hkv) & 1;
+        const int t0 = int(task / (2 * Hkv)) * WINDOW;
+        const long long pool = (long long)p.cache.num_pages * p.cache.page_size;
+        // Lane l holds the slot of token t - 15 + l (lane 31 none): the tokens
+        // that can share a block with t.
+        long long slot[WINDOW];
+#pragma unroll
+        for (int w = 0; w < WINDOW; ++w) {
+            const int tl = t0 + w - 15 + lane;
+            slot[w] = tl >= 0 && tl < p.T && lane < 31 ? p.slots[tl] : -1;
+        }
+        const __half* b = p.bias[1 + which];
+        Row8 bias = {};
+        if (b) bias = load_row<D>(b + (size_t)h * D, f0);
+#pragma unroll
+        for (int w = 0; w < WINDOW; ++w) {
+            const long long s = __shfl_sync(0xffffffffu, slot[w], 15);
+            if (s >= pool && lane == 15) record_error(p.err, kDevBadIndex);
+            if (s < 0 || s >= pool) continue;                       // uniform over the warp
+            const bool same = slot[w] >= 0 && slot[w] / kKv8Block == s / kKv8Block;
+            const uint32_t block = __ballot_sync(0xffffffffu, same);
+            if (block & 0x7fffu) continue;                          // an earlier token's warp has it
+            const long long before = __shfl_up_sync(0xffffffffu, slot[w], 1);
+            const uint32_t on = __ballot_sync(0xffffffffu, same && slot[w] == before + 1) >> 15;
+            uint32_t left = block >> 15;                            // bit j: token t + j
+            while (left) {
+                const int i = __ffs(left) - 1;
+                const int n = __ffs(~(on >> (i + 1)));              // 1 + the tokens that go on
+                left &= ~(((1u << n) - 1u) << i);
+                const long long si = __shfl_sync(0xffffffffu, slot[w], 15 + i);
+                append_run<D, Code>(p, which, h, t0 + w + i, n, si, bias, b != nullptr, lane);
+                __syncwarp();                                       // the next run of the block reads it
+            }
+        }
+        return;
+    }
+    const int chunks = (p.H + kQHeads - 1) / kQHeads;
+    const long long item = (task - kv_tasks) * RPW + lane / LPR;
+    if (item >= (long long)p.T * chunks) return;
+    const int t = int(item / chunks);
+    const int h0 = int(item - (long long)t * chunks) * kQHeads;
+    const long long slot = p.slots[t];
+    if (slot < 0) return;
+    const __half* src = p.q + (size_t)t * p.stride[0];
+    __half* dst = p.q_out + (size_t)t * p.stride[3];
+    Row8 r[kQHeads];
+#pragma unroll
+    for (int j = 0; j < kQHeads; ++j)
+        if (h0 + j < p.H) r[j] = load_row<D>(src + (size_t)(h0 + j) * D, f0);
+    float c[4], s[4];
+    load_turn<D>(p, t, f0, c, s);
+#pragma unroll
+    for (int j = 0; j < kQHeads; ++j)
+        if (h0 + j < p.H) {
+            if (p.bias[0]) add_bias(r[j], load_row<D>(p.bias[0] + (size_t)(h0 + j) * D, f0));
+            turn(r[j], c, s);
+            store_row<D>(dst + (size_t)(h0 + j) * D, f0, r[j]);
+        }
+}
+
+// ---------------------------------------------------------------------------
+// Read-back: out[i] = fp16(code * scale) of slot slots[i], every kv head; a
+// slot outside the pool gives zeros.  One thread widens 16 codes (a 16-byte
+// load) of K and of V; consecutive threads take consecutive pieces of the
+// output row, so both sides move whole sectors.  Bound by bytes.
+// ---------------------------------------------------------------------------
+struct GatherParams {
+    Kv8View cache;
+    const long long* slots;
+    __half* k_out;
+    __half* v_out;
+    long long pieces;                   // slots x Hkv x D / 16
+};
+
+template <class Code>
+__device__ __forceinline__ void widen16(uint4 w, float scale, __half* out) {
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    uint32_t h[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t x = Code::prepare(in[i]);
+        const uint32_t pair[2] = {Code::half2_lo(x), Code::half2_hi(x)};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pair[e]));
+            h[2 * i + e] = pack_half2(f.x * scale, f.y * scale);
+        }
+    }
+    uint4* o = reinterpret_cast<uint4*>(out);
+    o[0] = make_uint4(h[0], h[1], h[2], h[3]);
+    o[1] = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+template <int D, class Code>
+__global__ void __launch_bounds__(256)
+kv8_gather_kernel(const GatherParams p) {
+    constexpr int PPR = D / 16;                 // pieces per row
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= p.pieces) return;
+    const Kv8View& c = p.cache;
+    const int e = int(i % PPR) * 16;
+    const long long row = i / PPR;
+    const int h = int(row % c.Hkv);
+    const long long slot = p.slots[row / c.Hkv];
+    const bool real = slot >= 0 && slot < (long long)c.num_pages * c.page_size;
+    const int page = real ? int(slot / c.page_size) : 0;
+    const int r = real ? int(slot - (long long)page * c.page_size) : 0;
+    float2 scale = make_float2(0.f, 0.f);
+    uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
+    if (real) {
+        const size_t at = c.row(page, h, r) + e;
+        if (p.k_out) kw = *reinterpret_cast<const uint4*>(c.k + at);
+        if (p.v_out) vw = *reinterpret_cast<const uint4*>(c.v + at);
+        scale = *c.scale(page, h, r);
+    }
+    if (p.k_out) widen16<Code>(kw, scale.x, p.k_out + row * D + e);
+    if (p.v_out) widen16<Code>(vw, scale.y, p.v_out + row * D + e);
+}
+
+}  // namespace fr

@@ -245,6 +245,134 @@ FR_API int fr_qkv_bias_rope_append(void* q, void* k, void* v, const void* q_bias
 FR_API int fr_prefill_attn(const void* q, const void* k, const void* v, void* out, int seq_len,
                     int num_heads, int num_kv_heads, int head_dim, void* stream);
 
+/* ---- Serving from a paged cache held in 8 bits ---------------------------
+ * One step of a server, all on one stream and capturable in a CUDA graph:
+ *   fr_paged_step              pages, positions and slots of the step's tokens
+ *   per layer:
+ *   fr_qkv_rope_append_kv8     bias + RoPE on q/k, K/V coded into the cache
+ *   fr_decode_attn_paged_kv8   attention of one token per sequence over it
+ * No reference counterpart (one 16-bit contiguous cache per layer,
+ * runtime/kv_cache.cpp:14-37).
+ *
+ * A cached value is code * scale.  k and v hold one-byte codes for
+ * [num_pages][num_kv_heads][page_size][head_dim]; the last dimension is
+ * contiguous, the others have the strides given (in bytes, multiples of 16),
+ * so token-major pages or K and V interleaved in one allocation work too.
+ * One K and one V scale belong to each block of FR_KV8_BLOCK consecutive rows
+ * of a page and each kv head:
+ *   scales [num_pages][num_kv_heads][page_size / FR_KV8_BLOCK][2] fp32 (K, V)
+ * Slot s is row s % page_size of page s / page_size. */
+#define FR_KV8_INT8 0          /* codes -127 .. 127 */
+#define FR_KV8_E4M3 1          /* 4 exponent, 3 mantissa bits; largest 448 */
+#define FR_KV8_BLOCK 16
+
+typedef struct fr_kv8_cache {
+    void* k;                   /* 16-byte aligned */
+    void* v;
+    float* scales;             /* 8-byte aligned */
+    int dtype;                 /* FR_KV8_INT8 or FR_KV8_E4M3 */
+    int num_pages;
+    int page_size;             /* a multiple of FR_KV8_BLOCK rows */
+    int num_kv_heads;
+    int head_dim;              /* 64 or 128 */
+    long long page_stride;     /* bytes between pages, kv heads and rows */
+    long long head_stride;
+    long long row_stride;
+} fr_kv8_cache;
+
+/* Block tables and slot maps of one step, on the GPU, from request lengths.
+ *   kv_lens     [batch] tokens each request holds, in the first
+ *               ceil(kv_lens[b] / page_size) entries of its block-table row
+ *   new_lens    [batch] tokens it gets in this step (0: none); a negative
+ *               number ends the request: its pages go back, its length is 0
+ *   block_table [batch, max_blocks_per_seq], extended in place
+ *   free_pages  [num_pages] stack of page ids, the first *free_count of them
+ *               free; the ended requests' pages are pushed in (request, block)
+ *               order, then the new pages popped from the top in (request,
+ *               block) order.  Entries from free_count_out on are left as
+ *               pushed.
+ *   kv_lens_out, free_count_out   the values after the step (may be kv_lens
+ *               and free_count: updated in place)
+ *   token_offsets [batch + 1]  exclusive prefix sum of the new tokens
+ *   positions, slots [max_tokens] of each new token, in request order; past
+ *               the last one, position 0 and slot -1 (a call captured in a
+ *               graph can run fewer tokens than it was sized for)
+ *   status      [1] device word: FR_STEP_OK, or why the step was refused.  A
+ *               refused step changes nothing: lengths, table and stack stay,
+ *               offsets and positions are 0, every slot is -1.
+ * All arrays int32 but slots (int64), all on the device.  batch <= 8192,
+ * max_tokens, num_pages and max_blocks_per_seq * page_size below 2^30. */
+#define FR_STEP_OK 0
+#define FR_STEP_NO_PAGES 1     /* more pages needed than are free or released */
+#define FR_STEP_BAD_LENGTH 2   /* a length below 0 or past the block-table row */
+#define FR_STEP_TOO_MANY 3     /* more new tokens than max_tokens */
+#define FR_STEP_BAD_FREE 4     /* free_count outside the stack, or it would overflow */
+FR_API int fr_paged_step(const int* kv_lens, const int* new_lens, int* block_table,
+                         int* free_pages, const int* free_count, int* kv_lens_out,
+                         int* free_count_out, int* token_offsets, int* positions,
+                         long long* slots, int* status, int batch, int page_size, int num_pages,
+                         int max_blocks_per_seq, int max_tokens, void* stream);
+
+/* Prologue of the 8-bit cache, one launch: q/k/v bias, NeoX RoPE on q and k,
+ * K and V coded into the cache at the tokens' slots.  All arithmetic in fp32;
+ * q_out, k_out and v_out are rounded to fp16 once.
+ *   q [num_tokens, num_heads, head_dim], k, v [num_tokens, num_kv_heads, head_dim] fp16
+ *   q_out       may be q; k_out, v_out: NULL (decode: only the cache is
+ *               needed) or a buffer, which may be k, v (prefill attention)
+ *   token_strides  host array of 6: halves between consecutive tokens of q,
+ *               k, v, q_out, k_out, v_out (multiples of 4); NULL = contiguous
+ *   *_bias      fp16 [heads * head_dim] or NULL
+ *   cos_tab, sin_tab  [table_rows, head_dim / 2] fp32 (fr_rope_tables)
+ *   positions   int32 [num_axes, num_tokens]; frequency f turns by table row
+ *               positions[freq_axis[f]] (rotary positions with several axes,
+ *               e.g. time, height and width of image patches).  num_axes 1..4;
+ *               freq_axis: host array of head_dim / 2 bytes, NULL with one axis
+ *   slots       int64 [num_tokens]; a token whose slot is negative is left
+ *               out (none of its outputs is written)
+ * Scales: consecutive tokens of a call in consecutive rows of one block are
+ * coded together with scale amax / (127 or 448), at least the block's old
+ * scale if they do not start at its row 0 (the rows below them are then taken
+ * to be held); if the scale grows, those rows are coded anew.  A call's tokens
+ * of one block lie within 16 consecutive tokens, as fr_paged_step lays them
+ * out, and are taken in token order.  A block that holds a NaN or an infinity reads back as NaN.
+ * A position outside the table (read as 0) or a slot outside the pool (not
+ * cached) is recorded: fr_get_device_error then gives device code 4 and
+ * FR_ERR_INVALID_ARG.  num_tokens 0 does nothing. */
+FR_API int fr_qkv_rope_append_kv8(const void* q, const void* k, const void* v, void* q_out,
+                                  void* k_out, void* v_out, const long long* token_strides,
+                                  const void* q_bias, const void* k_bias, const void* v_bias,
+                                  const float* cos_tab, const float* sin_tab, int table_rows,
+                                  const int* positions, int num_axes,
+                                  const unsigned char* freq_axis, const long long* slots,
+                                  const fr_kv8_cache* cache, int num_tokens, int num_heads,
+                                  void* stream);
+
+/* Reads slots back as fp16: k_out, v_out [num_slots, num_kv_heads, head_dim]
+ * (16-byte aligned; either may be NULL), e.g. a cached prefix for the 16-bit
+ * prefill attention.  A slot outside the pool gives zeros. */
+FR_API int fr_kv8_gather(const fr_kv8_cache* cache, const long long* slots, void* k_out,
+                         void* v_out, int num_slots, void* stream);
+
+/* Decode attention over the 8-bit paged cache, one token per sequence.
+ *   q            [batch, num_heads, head_dim] fp16, q_stride halves between
+ *                sequences (a multiple of 8; 0 = num_heads * head_dim), 16-byte aligned
+ *   out          [batch, num_heads, head_dim] fp16, 16-byte aligned
+ *   block_table  device int32 [batch, max_blocks_per_seq]; page ids outside
+ *                the pool read as zero rows
+ *   kv_lens      device int32 [batch]; 0 yields zeros, a length above
+ *                max_kv_len is cut to it
+ *   max_kv_len   host upper bound of kv_lens, <= max_blocks_per_seq * page_size
+ * Rows past a sequence's end are never used, whatever they hold.  A NaN or
+ * infinite scale of a used block makes the outputs it enters NaN.  The result
+ * does not depend on which CTA merges: equal inputs give equal bits. */
+FR_API int fr_decode_attn_paged_kv8(const void* q, long long q_stride, const fr_kv8_cache* cache,
+                                    const int* block_table, const int* kv_lens, void* out,
+                                    int batch, int num_heads, int max_blocks_per_seq,
+                                    int max_kv_len, void* stream);
+/* Workspace bytes one such call uses (see fr_reserve_workspace). */
+FR_API size_t fr_kv8_workspace_size(int batch, int num_heads, int num_kv_heads, int head_dim,
+                                    int max_kv_len);
+
 /* Grows the current device's workspace to at least `bytes` (call before
  * CUDA-graph capture).  fr_decode_workspace_size() gives the bytes one call
  * of fr_decode_attn_batched with these sizes needs (fr_decode_attn: batch 1). */
@@ -261,8 +389,8 @@ FR_API size_t fr_prefill_workspace_size(int seq_len, int num_heads, int head_dim
 
 /* Reads (and optionally clears) the current device's in-kernel error words
  * (the regular entry points' and fr_decode_attn_noalloc's): 0 = none,
- * otherwise a bounded wait ran out (FR_ERR_TIMEOUT is returned by the
- * status).  Synchronises the device; creates no state and allocates
+ * 4 = an index out of range (fr_qkv_rope_append_kv8; FR_ERR_INVALID_ARG is
+ * returned), otherwise a bounded wait ran out (FR_ERR_TIMEOUT is returned).  Synchronises the device; creates no state and allocates
  * nothing. */
 FR_API int fr_get_device_error(int clear, int* device_code);
 
