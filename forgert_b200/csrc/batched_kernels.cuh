@@ -72,8 +72,8 @@ struct PersistSmem {
 };
 
 // Tiles per sequence (at least one) as an exclusive prefix in unit tiles
-// (x upb units per sequence): seq_start[0..B]; lens[b] = kv_lens[b], at most cap.  Every
-// thread of the block takes part.
+// (x upb units per sequence): seq_start[0..B]; lens[b] = kv_lens[b], at most
+// cap.  Every thread of the block takes part.
 template <int TILE>
 __device__ __forceinline__ void scan_lengths(const int* kv_lens, int B, int upb, int* seq_start,
                                              int* lens, int* warp_sums, int cap = 0x7fffffff) {
@@ -210,16 +210,7 @@ struct CostMap {
 // fragments with FMAs only.  The order of the sums is fixed (contributor
 // order within a lane group, lanes by shuffle tree), so the result does not
 // depend on which CTA merges.  All consumer threads take part.
-//
-// Dims names the head dimension of component c of a fragment: MmaDims is the
-// layout above, with which the fp16 rows of the cache come out of ldmatrix.
-template <int D>
-struct MmaDims {
-    static __device__ __forceinline__ int dim(int dm, int g, int c) { return dm * 16 + g + ((c >> 1) << 3); }
-    static __device__ __forceinline__ float inverse(float l) { return l > 0.f ? 1.f / l : 0.f; }
-};
-
-template <int D, int NT, int NW, class Dims = MmaDims<D>>
+template <int D, int NT, int NW>
 __device__ __forceinline__ void merge_pieces(const DecodeParams& p, float* area, int cf, int cl,
                                              bool cf_tail, int gcount, size_t head_base) {
     constexpr int GP = NT * 8;
@@ -283,7 +274,7 @@ __device__ __forceinline__ void merge_pieces(const DecodeParams& p, float* area,
         sm_w[wu * GP + wh] = w;
         if (wu == 0) {
             sm_r[wh] = r;
-            sm_inv[wh] = Dims::inverse(lrun);
+            sm_inv[wh] = lrun > 0.f ? 1.f / lrun : 0.f;
         }
         consumer_sync(NTHR);
         if (tid == 0) FR_TRACE_EV(kEvMergeLoaded);
@@ -312,13 +303,13 @@ __device__ __forceinline__ void merge_pieces(const DecodeParams& p, float* area,
 #pragma unroll
     for (int i = 0; i < FPT; ++i) {
         const int f = tid + i * NTHR;
-        const int dm = f / (32 * NT), g = (f & 31) >> 2;
+        const int d = (f / (32 * NT)) * 16 + ((f & 31) >> 2);
         const float vals[4] = {acc[i].x, acc[i].y, acc[i].z, acc[i].w};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             const int h = ha[i] + (c & 1);
             if (h < gcount)
-                p.out[(head_base + h) * D + Dims::dim(dm, g, c)] = __float2half_rn(vals[c] * sm_inv[h]);
+                p.out[(head_base + h) * D + d + ((c >> 1) << 3)] = __float2half_rn(vals[c] * sm_inv[h]);
         }
     }
 }

@@ -276,10 +276,21 @@ __device__ __forceinline__ void cp_async_8(uint32_t dst_smem, const void* src, u
                  :: "r"(dst_smem), "l"(src), "r"(src_bytes) : "memory");
 }
 
-// Arrives on `bar` once this thread's earlier cp.async copies have landed.
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];"
-                 :: "r"(smem_u32(bar)) : "memory");
+// 16-byte copy into shared memory past L1, with an L2 policy.
+__device__ __forceinline__ void cp_async_16(uint32_t dst_smem, const void* src, uint32_t src_bytes,
+                                            uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint.L2::128B [%0], [%1], 16, %2, %3;"
+                 :: "r"(dst_smem), "l"(src), "r"(src_bytes), "l"(policy) : "memory");
+}
+
+__device__ __forceinline__ void cp_async_commit() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+// Waits until at most N of this thread's newest groups are under way.
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory");
 }
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -336,6 +347,13 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// log2(x) with the hardware approximation (MUFU.LG2); fast_log2(0) = -inf.
+__device__ __forceinline__ float fast_log2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 

@@ -20,7 +20,7 @@ int check_kv8(const fr_kv8_cache* c) {
         (c->dtype != FR_KV8_INT8 && c->dtype != FR_KV8_E4M3))
         return FR_ERR_INVALID_ARG;
     if (c->head_dim != 64 && c->head_dim != 128) return FR_ERR_UNSUPPORTED;
-    const long long limit = 1LL << 40;           // of a tensor map's strides
+    const long long limit = 1LL << 40;
     for (long long s : {c->page_stride, c->head_stride, c->row_stride})
         if (s < c->head_dim || s >= limit) return FR_ERR_INVALID_ARG;
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->scales, 8) ||
@@ -43,41 +43,23 @@ fr::Kv8View kv8_view(const fr_kv8_cache* c) {
     return v;
 }
 
-// K or V codes as a 4-D tensor [num_pages][Hkv][page_size][D] of bytes, box =
-// `box` rows of one kv head of one page, swizzled by the row's width (128 or
-// 64 bytes).  A page index past the pool reads as zeros.
-int encode_kv8_map(CUtensorMap* map, const void* base, const fr_kv8_cache* c, int box) {
-    auto fn = encode_fn();
-    if (!fn) return cuda_fail(cudaErrorNotSupported);
-    const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size,
-                                (cuuint64_t)c->num_kv_heads, (cuuint64_t)c->num_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)c->row_stride, (cuuint64_t)c->head_stride,
-                                   (cuuint64_t)c->page_stride};
-    const cuuint32_t boxes[4] = {(cuuint32_t)c->head_dim, (cuuint32_t)box, 1, 1};
-    const cuuint32_t estr[4] = {1, 1, 1, 1};
-    static const int promo = env_int("FORGERT_L2_PROMO", 3);
-    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides,
-                    boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    c->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                    static_cast<CUtensorMapL2promotion>(promo & 3),
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? FR_OK : cuda_fail(cudaErrorInvalidValue);
-}
-
-// Tiles of 128 positions: four consumer warps of two m-tiles.  Stages of
-// 32 KB (D = 128) or 16 KB (D = 64), 96 KB in flight per CTA, two CTAs per SM.
-constexpr int kKv8Mt = 2;
+// Shape of the decode kernel: four warps, steps of 16 (D = 128) or 32 (D = 64)
+// rows, 4 KB of codes.  Up to 8 query heads per kv head: four CTAs per SM (128
+// registers) and two steps under way per warp; more: three CTAs (168 registers,
+// the second 8-head tile's state spills at 128) and three steps.
 constexpr int kKv8Warps = 4;
-constexpr int kKv8Ctas = 2;
-constexpr int kKv8Tile = 16 * kKv8Mt * kKv8Warps;
-template <int D> constexpr int kv8_stages() { return D == 64 ? 6 : 3; }
+template <int NT> constexpr int kv8_ctas() { return NT == 1 ? 4 : 3; }
+template <int NT> constexpr int kv8_stages() { return NT == 1 ? 2 : 3; }
+template <int D> constexpr int kv8_mt() { return 128 / D; }
+constexpr int kv8_tile(int head_dim) { return 16 * (128 / head_dim) * kKv8Warps; }
 
 template <int D, int NT>
-using Kv8SmemOf = fr::Kv8Smem<D, NT, kKv8Tile, kv8_stages<D>(), kKv8Warps>;
+using Kv8SmemOf = fr::Kv8Smem<D, NT, kv8_mt<D>(), kv8_stages<NT>(), kKv8Warps>;
 
 template <int D, int NT, class Code>
 auto kv8_ptr() {
-    return fr::kv8_decode_kernel<D, NT, kKv8Mt, kv8_stages<D>(), kKv8Warps, kKv8Ctas, Code>;
+    return fr::kv8_decode_kernel<D, NT, kv8_mt<D>(), kv8_stages<NT>(), kKv8Warps, kv8_ctas<NT>(),
+                                 Code>;
 }
 
 template <int D, int NT, class Code>
@@ -90,7 +72,7 @@ int prepare_kv8(DeviceState* st, int slot) {
     if (e != cudaSuccess) return cuda_fail(e);
     int n = 0;
     e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv8_ptr<D, NT, Code>(),
-                                                      32 * (kKv8Warps + 1), bytes);
+                                                      32 * kKv8Warps, bytes);
     if (e != cudaSuccess) return cuda_fail(e);
     st->kv8_occ[slot] = std::max(1, n);
     return FR_OK;
@@ -100,14 +82,14 @@ template <int D, int NT, class Code>
 int launch_kv8(const fr::Kv8DecodeParams& kp, int ctas, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, 1, 1);
-    cfg.blockDim = dim3(32 * (kKv8Warps + 1), 1, 1);
+    cfg.blockDim = dim3(32 * kKv8Warps, 1, 1);
     cfg.dynamicSmemBytes = Kv8SmemOf<D, NT>::kBytes;
     cfg.stream = s;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = s != nullptr ? 1 : 0;
+    cfg.numAttrs = 1;
     cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_ptr<D, NT, Code>(), kp);
     g_launches.fetch_add(1, std::memory_order_relaxed);
     if (e == cudaSuccess) e = cudaGetLastError();
@@ -129,13 +111,17 @@ int kv8_dispatch(int head_dim, int nt, int dtype, F f) {
                           : with_nt(integral_constant<int, 128>());
 }
 
+// Counters of a call: one per unit, then one per partial slot.
+constexpr int kKv8Units = kMaxUnits / 2;
+
 // Sequences per launch: their lengths' prefix fits shared memory, their units
 // the counters, their tiles the kernel's 32-bit tile numbers.  0 = not even one.
-int kv8_chunk(int batch, int num_kv_heads, int head_groups, int max_kv_len) {
+int kv8_chunk(int batch, int num_kv_heads, int head_groups, int head_dim, int max_kv_len) {
     const long long upb = (long long)num_kv_heads * head_groups;
-    const long long tiles = std::max(1, (max_kv_len + kKv8Tile - 1) / kKv8Tile);
-    const long long n = std::min({(long long)fr::kPersistMaxBatch, kMaxUnits / upb,
-                                  ((1LL << 30) - 1) / (upb * tiles), (long long)batch});
+    const int tile = kv8_tile(head_dim);
+    const long long tiles = std::max(1, (max_kv_len + tile - 1) / tile);
+    const long long n = std::min({(long long)fr::kPersistMaxBatch, kKv8Units / upb,
+                                  ((1LL << 29) - 1) / (upb * tiles), (long long)batch});
     return (int)n;
 }
 
@@ -150,15 +136,16 @@ int kv8_plan(DeviceState* st, int batch, int num_heads, int num_kv_heads, int he
     const int group = num_heads / num_kv_heads;
     pl.nt = group <= 8 ? 1 : 2;
     pl.head_groups = (group + 8 * pl.nt - 1) / (8 * pl.nt);
-    pl.chunk = kv8_chunk(batch, num_kv_heads, pl.head_groups, max_kv_len);
+    pl.chunk = kv8_chunk(batch, num_kv_heads, pl.head_groups, head_dim, max_kv_len);
     if (pl.chunk <= 0) return FR_ERR_INVALID_ARG;
     const int slot = (head_dim == 64 ? 0 : 4) + (pl.nt - 1) * 2 + dtype;
     int rc = kv8_dispatch(head_dim, pl.nt, dtype, [&](auto d, auto n, auto code) {
         return prepare_kv8<decltype(d)::value, decltype(n)::value, decltype(code)>(st, slot);
     });
     if (rc != FR_OK) return rc;
+    const int tile = kv8_tile(head_dim);
     const long long tiles = (long long)pl.chunk * num_kv_heads * pl.head_groups *
-                            std::max(1, (max_kv_len + kKv8Tile - 1) / kKv8Tile);
+                            std::max(1, (max_kv_len + tile - 1) / tile);
     pl.ctas = (int)std::max<long long>(
         1, std::min<long long>((long long)st->sm_count * st->kv8_occ[slot], tiles));
     pl.ws_bytes = kCounterBytes + (size_t)2 * pl.ctas * 8 * pl.nt * (head_dim + 2) * sizeof(float);
@@ -179,36 +166,28 @@ int run_kv8(const void* q, long long q_stride, const fr_kv8_cache* cache, const 
     if (rc != FR_OK) return rc;
     rc = ensure_workspace(st, pl.ws_bytes, s);
     if (rc != FR_OK) return rc;
-    fr::Kv8DecodeParams kp;
-    std::memset(&kp, 0, sizeof(kp));
-    DecodeParams& p = kp.d;
-    const int box = std::gcd(cache->page_size, kKv8Tile);    // a box never straddles a page
-    rc = encode_kv8_map(&p.kmap, cache->k, cache, box);
-    if (rc == FR_OK) rc = encode_kv8_map(&p.vmap, cache->v, cache, box);
-    if (rc != FR_OK) return rc;
+    fr::Kv8DecodeParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.cache = kv8_view(cache);
+    p.q_stride = q_stride;
     p.H = num_heads;
-    p.Hkv = Hkv;
     p.G = num_heads / Hkv;
     p.head_groups = pl.head_groups;
+    p.bt_stride = max_blocks;
+    p.max_len = max_kv_len;
     p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)D));
-    p.err = st->err;
     p.counters = static_cast<int*>(st->ws);
+    p.max_units = kKv8Units;
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(st->ws) + kCounterBytes);
     p.part_acc = p.part_ml + (size_t)2 * pl.ctas * 8 * pl.nt * 2;
-    static const int evict_normal = env_int("FORGERT_EVICT_NORMAL", 0);
-    p.evict_normal = evict_normal;
-    p.min_tiles_per_cta = 8;
+    // At least four tiles per CTA before SMs get more than one; a unit's start
+    // and its merge are charged as one tile each (four each, which suits the
+    // 16-bit kernel's longer tiles, left too few CTAs to short calls: one
+    // sequence of 2048 tokens 18.6 us instead of 10.6).
+    p.min_tiles_per_cta = 4;
     p.min_ctas = st->sm_count;
-    p.item_cost = 4;
-    p.merge_cost = 4;
-    p.bt_stride = max_blocks;
-    p.page_size = cache->page_size;
-    p.page_box = box;
-    p.num_pages = cache->num_pages;
-    kp.scales = cache->scales;
-    kp.blocks_per_page = cache->page_size / fr::kKv8Block;
-    kp.max_len = max_kv_len;
-    kp.q_stride = q_stride;
+    p.item_cost = 1;
+    p.merge_cost = 1;
     for (int b = 0; b < batch; b += pl.chunk) {
         p.batch = std::min(pl.chunk, batch - b);
         p.q = static_cast<const __half*>(q) + (size_t)b * q_stride;
@@ -216,17 +195,19 @@ int run_kv8(const void* q, long long q_stride, const fr_kv8_cache* cache, const 
         p.kv_lens = kv_lens + b;
         p.block_table = block_table + (size_t)b * max_blocks;
         rc = kv8_dispatch(D, pl.nt, cache->dtype, [&](auto d, auto n, auto code) {
-            return launch_kv8<decltype(d)::value, decltype(n)::value, decltype(code)>(kp, pl.ctas,
-                                                                                     s);
+            return launch_kv8<decltype(d)::value, decltype(n)::value, decltype(code)>(p, pl.ctas, s);
         });
         if (rc != FR_OK) return rc;
     }
     return FR_OK;
 }
 
+// Programmatic dependent launch, on the default stream too: every kernel here
+// waits for the grid before it ahead of its first access to memory, so only
+// the launch itself overlaps (1.5 to 2 us a call).
 template <class... Args>
 int launch_plain(void (*fn)(Args...), unsigned grid, unsigned block, size_t smem, cudaStream_t s,
-                 bool pdl, Args... args) {
+                 Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid, 1, 1);
     cfg.blockDim = dim3(block, 1, 1);
@@ -236,7 +217,7 @@ int launch_plain(void (*fn)(Args...), unsigned grid, unsigned block, size_t smem
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = pdl && s != nullptr ? 1 : 0;
+    cfg.numAttrs = 1;
     cudaError_t e = cudaLaunchKernelEx(&cfg, fn, args...);
     g_launches.fetch_add(1, std::memory_order_relaxed);
     if (e == cudaSuccess) e = cudaGetLastError();
@@ -295,7 +276,7 @@ int fr_paged_step(const int* kv_lens, const int* new_lens, int* block_table, int
             else p.ticket = static_cast<int*>(st->ws);
         }
         return launch_plain(fr::paged_step_kernel, (unsigned)ctas, fr::kStepThreads, smem, s,
-                            false, static_cast<const fr::StepParams>(p));
+                            static_cast<const fr::StepParams>(p));
     });
 }
 
@@ -373,7 +354,7 @@ int fr_qkv_rope_append_kv8(const void* q, const void* k, const void* v, void* q_
         return kv8_dispatch(D, 1, cache->dtype, [&](auto d, auto, auto code) {
             auto fn = window == 1 ? fr::kv8_append_kernel<decltype(d)::value, 1, decltype(code)>
                                   : fr::kv8_append_kernel<decltype(d)::value, 4, decltype(code)>;
-            return launch_plain(fn, (unsigned)grid, fr::kAppendThreads, 0, s, true,
+            return launch_plain(fn, (unsigned)grid, fr::kAppendThreads, 0, s,
                                 static_cast<const fr::AppendParams>(p));
         });
     });
@@ -398,7 +379,7 @@ int fr_kv8_gather(const fr_kv8_cache* cache, const long long* slots, void* k_out
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         return kv8_dispatch(cache->head_dim, 1, cache->dtype, [&](auto d, auto, auto code) {
             return launch_plain(fr::kv8_gather_kernel<decltype(d)::value, decltype(code)>,
-                                (unsigned)grid, 256, 0, s, true,
+                                (unsigned)grid, 256, 0, s,
                                 static_cast<const fr::GatherParams>(p));
         });
     });

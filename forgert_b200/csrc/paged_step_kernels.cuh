@@ -78,6 +78,8 @@ paged_step_kernel(const StepParams p) {
     const int cap[3] = {p.max_tokens + 1, p.num_pages + 1, p.num_pages + 1};
     const long long most = (long long)p.max_blocks * P;
 
+    grid_launch_dependents();
+    grid_dependency_wait();
     const int count = *p.free_count;
     int carry[3] = {0, 0, 0};
     int bad = 0;
