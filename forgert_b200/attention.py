@@ -30,6 +30,11 @@ __all__ = [
 def _ptr(x) -> int | None:
     if x is None:
         return None
+    try:                                # the common case first: this is most of a call's host time
+        if x.is_cuda:
+            return x.data_ptr()
+    except AttributeError:
+        pass
     if isinstance(x, int):
         return x
     dp = getattr(x, "data_ptr", None)
@@ -233,11 +238,13 @@ def paged_step(kv_lens, new_lens, block_table, free_pages, free_count, kv_lens_o
     token_offsets [batch + 1], positions / slots (int64) [max_tokens].  status
     [1] is FR_STEP_OK, or why the step was refused and nothing changed."""
     lib = load()
-    check("fr_paged_step", lib.fr_paged_step(
+    rc = lib.fr_paged_step(
         _ptr(kv_lens), _ptr(new_lens), _ptr(block_table), _ptr(free_pages), _ptr(free_count),
         _ptr(kv_lens_out), _ptr(free_count_out), _ptr(token_offsets), _ptr(positions),
         _ptr(slots), _ptr(status), batch, page_size, num_pages, max_blocks_per_seq, max_tokens,
-        _stream(stream)))
+        _stream(stream))
+    if rc:
+        check("fr_paged_step", rc)
 
 
 def qkv_rope_append_kv8(q, k, v, q_out, k_out, v_out, cos_tab, sin_tab, positions, slots,
@@ -255,18 +262,22 @@ def qkv_rope_append_kv8(q, k, v, q_out, k_out, v_out, cos_tab, sin_tab, position
     strides = None
     if token_strides is not None:
         strides = (ctypes.c_longlong * 6)(*token_strides)
-    check("fr_qkv_rope_append_kv8", lib.fr_qkv_rope_append_kv8(
+    rc = lib.fr_qkv_rope_append_kv8(
         _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(v_out), strides, _ptr(q_bias),
         _ptr(k_bias), _ptr(v_bias), _ptr(cos_tab), _ptr(sin_tab), table_rows, _ptr(positions),
-        num_axes, freq_axis, _ptr(slots), cache._ref, num_tokens, num_heads, _stream(stream)))
+        num_axes, freq_axis, _ptr(slots), cache._ref, num_tokens, num_heads, _stream(stream))
+    if rc:
+        check("fr_qkv_rope_append_kv8", rc)
 
 
 def kv8_gather(cache: KV8Cache, slots, k_out, v_out, num_slots: int, stream=None) -> None:
     """Reads slots back as fp16 [num_slots, num_kv_heads, head_dim] (either
     output may be None); a slot outside the pool gives zeros."""
     lib = load()
-    check("fr_kv8_gather", lib.fr_kv8_gather(cache._ref, _ptr(slots), _ptr(k_out), _ptr(v_out),
-                                             num_slots, _stream(stream)))
+    rc = lib.fr_kv8_gather(cache._ref, _ptr(slots), _ptr(k_out), _ptr(v_out),
+                           num_slots, _stream(stream))
+    if rc:
+        check("fr_kv8_gather", rc)
 
 
 def decode_attn_paged_kv8(q, cache: KV8Cache, block_table, kv_lens, out, batch: int,
@@ -277,9 +288,11 @@ def decode_attn_paged_kv8(q, cache: KV8Cache, block_table, kv_lens, out, batch: 
     sequences' q, 0 = contiguous), block_table int32 [batch,
     max_blocks_per_seq], kv_lens int32 [batch]."""
     lib = load()
-    check("fr_decode_attn_paged_kv8", lib.fr_decode_attn_paged_kv8(
+    rc = lib.fr_decode_attn_paged_kv8(
         _ptr(q), q_stride, cache._ref, _ptr(block_table), _ptr(kv_lens), _ptr(out), batch,
-        num_heads, max_blocks_per_seq, max_kv_len, _stream(stream)))
+        num_heads, max_blocks_per_seq, max_kv_len, _stream(stream))
+    if rc:
+        check("fr_decode_attn_paged_kv8", rc)
 
 
 def kv8_workspace_size(batch: int, num_heads: int, num_kv_heads: int, head_dim: int,

@@ -303,6 +303,8 @@ int fr_qkv_rope_append_kv8(const void* q, const void* k, const void* v, void* q_
             if (freq_axis[f] >= num_axes) return FR_ERR_INVALID_ARG;
             p.axis[f] = freq_axis[f];
         }
+    p.by_quads = 1;
+    for (int f = 0; f < D / 2; ++f) p.by_quads &= p.axis[f] == p.axis[f & ~3];
     const long long heads[6] = {num_heads, Hkv, Hkv, num_heads, Hkv, Hkv};
     for (int i = 0; i < 6; ++i) {
         p.stride[i] = token_strides ? token_strides[i] : heads[i] * D;
@@ -337,23 +339,29 @@ int fr_qkv_rope_append_kv8(const void* q, const void* k, const void* v, void* q_
         p.err = st->err;
         p.T = num_tokens;
         p.H = num_heads;
-        p.axes = num_axes;
         p.table_rows = table_rows;
-        // A warp per token while that fills the SMs' warps about once (a
-        // decode step's tokens are blocks of their own); four tokens a warp for
-        // more, where most tokens share the block of one before them.
-        const long long singles = 2LL * num_tokens * Hkv;
-        const int window = singles <= 64LL * st->sm_count ? 1 : 4;
-        const int rows = 32 / (D / 8);               // lane groups of a warp
-        const long long kv_tasks = 2LL * ((num_tokens + window - 1) / window) * Hkv;
-        const long long items = (long long)num_tokens * ((num_heads + fr::kQHeads - 1) / fr::kQHeads);
-        const long long warps = kv_tasks + (items + rows - 1) / rows;
-        const long long per = fr::kAppendThreads / 32, grid = (warps + per - 1) / per;
+        // A CTA per token while the SMs hold them all (a decode step's tokens
+        // are blocks of their own, done one after the other in a window);
+        // windows of 4 and of 16 tokens for more, where most tokens share the
+        // block of one before them and their CTAs would have nothing to do
+        // (28 / 4 heads of 128, windows 1 / 4 / 16: 512 decoding sequences 15.4
+        // / 12.6 / 36.4 us, 2048 prompt tokens 25.0 / 13.5 / 11.0, 8192 prompt
+        // tokens 93 / 49 / 40).
+        const long long held = 16LL * st->sm_count, kv = 2LL * num_tokens * Hkv;
+        p.window = kv <= held ? 1 : kv <= 8 * held ? 4 : 16;
+        const long long kv_ctas = 2LL * ((num_tokens + p.window - 1) / p.window) * Hkv;
+        // Query heads of a token in one lane group, which looks its angles up
+        // once: four, more when the tokens alone fill the SMs.
+        const int rows = 32 / (D / 8) * fr::kAppendWarps;                  // lane groups of a CTA
+        const long long fit = std::max(1LL, held * rows / num_tokens);     // lane groups per token
+        p.q_heads = (int)std::max<long long>(4, (num_heads + fit - 1) / fit);
+        const long long items = (long long)num_tokens * ((num_heads + p.q_heads - 1) / p.q_heads);
+        const long long grid = kv_ctas + (items + rows - 1) / rows;
+        p.kv_ctas = (int)kv_ctas;
         if (grid >= (1LL << 31)) return FR_ERR_INVALID_ARG;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         return kv8_dispatch(D, 1, cache->dtype, [&](auto d, auto, auto code) {
-            auto fn = window == 1 ? fr::kv8_append_kernel<decltype(d)::value, 1, decltype(code)>
-                                  : fr::kv8_append_kernel<decltype(d)::value, 4, decltype(code)>;
+            auto fn = fr::kv8_append_kernel<decltype(d)::value, decltype(code)>;
             return launch_plain(fn, (unsigned)grid, fr::kAppendThreads, 0, s,
                                 static_cast<const fr::AppendParams>(p));
         });

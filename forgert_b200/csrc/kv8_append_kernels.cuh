@@ -11,16 +11,21 @@
 //   start the block;  code = round(x / scale), ties to even.
 // If that makes the scale grow, the block's earlier rows are coded anew:
 // code' = round(code * old / scale).  All runs of a block are the work of the
-// warp of its first token, in token order (more than one where a token between
+// CTA of its first token, in token order (more than one where a token between
 // them is left out), so the scale, the old rows and the new ones need no order
-// between warps.  The maximum is
-// taken over the bit patterns of |x|, where NaN is the largest: a block that
-// holds a NaN or an infinity gets such a scale and reads back as such.
+// between CTAs.  The maximum is taken over the bit patterns of |x|, where NaN
+// is the largest: a block that holds a NaN or an infinity gets such a scale and
+// reads back as NaN.
 //
 // Layout: LPR = D / 8 lanes share a row, lane l holding the pairs f = 4l ..
-// 4l + 3: 8-byte loads of both halves, 4-byte code stores, a 16-byte load
-// each of cosines and sines.  A warp holds a whole 16-row run in registers
-// (every row's loads in flight at once) and so reads it once.
+// 4l + 3: 8-byte loads of both halves, 4-byte code stores, a 16-byte load each
+// of cosines and sines.  The four warps of a CTA share a run's 16 rows, which
+// stay in registers (two rows' eighths a lane) from the load to the codes.
+// (One warp per run, 64 values a lane: 128 registers and straight-line code
+// that the instruction cache lost, 60 us for 4600 tokens of 28 / 4 heads.)
+//
+// Bound: bytes moved for prompts, latency (dependent rounds of loads) for a
+// decode step.
 #pragma once
 #include "fr_ptx.cuh"
 #include "decode_kernels.cuh"
@@ -31,7 +36,8 @@ namespace fr {
 
 constexpr int kAppendThreads = 128;
 constexpr int kMaxAxes = 4;
-constexpr int kQHeads = 4;              // query heads of a token that one lane group turns
+constexpr int kAppendWarps = kAppendThreads / 32;
+constexpr int kQHeads = 4;              // query rows that a lane has under way
 
 struct AppendParams {
     const __half* q;
@@ -48,7 +54,11 @@ struct AppendParams {
     const long long* slots;
     Kv8View cache;
     int* err;
-    int T, H, axes, table_rows;
+    int T, H, table_rows;
+    int window;                         // tokens that a K/V CTA looks through, at most 16
+    int q_heads;                        // query heads of a token that one lane group turns
+    int by_quads;                       // every group of four frequencies has one axis
+    int kv_ctas;
     uint8_t axis[64];                   // axis of frequency f
 };
 
@@ -82,32 +92,35 @@ __device__ __forceinline__ void store_row(__half* row, int f0, const Row8& r) {
 }
 
 // Cosines and sines of token t at the lane's four frequencies.  A position
-// outside the table is recorded and read as position 0.
+// outside the table is recorded and read as position 0.  By quads: each group
+// of four frequencies turns by one axis, so a lane looks up one position.
 template <int D>
 __device__ __forceinline__ void load_turn(const AppendParams& p, int t, int f0, float (&c)[4],
                                           float (&s)[4]) {
     constexpr int kHalf = D / 2;
     auto at = [&](int axis) {
         int pos = p.positions[(size_t)axis * p.T + t];
-        if (pos < 0 || pos >= p.table_rows) {
+        if ((unsigned)pos >= (unsigned)p.table_rows) {
             record_error(p.err, kDevBadIndex);
             pos = 0;
         }
         return pos;
     };
-    if (p.axes == 1) {
-        const size_t e = (size_t)at(0) * kHalf + f0;
+    if (p.by_quads) {
+        const size_t e = (size_t)at(p.axis[f0]) * kHalf + f0;
         const float4 cv = *reinterpret_cast<const float4*>(p.cos_tab + e);
         const float4 sv = *reinterpret_cast<const float4*>(p.sin_tab + e);
         c[0] = cv.x; c[1] = cv.y; c[2] = cv.z; c[3] = cv.w;
         s[0] = sv.x; s[1] = sv.y; s[2] = sv.z; s[3] = sv.w;
         return;
     }
-#pragma unroll
+#pragma unroll 1
     for (int j = 0; j < 4; ++j) {
         const size_t e = (size_t)at(p.axis[f0 + j]) * kHalf + f0 + j;
-        c[j] = p.cos_tab[e];
-        s[j] = p.sin_tab[e];
+        const float cj = p.cos_tab[e], sj = p.sin_tab[e];
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            if (x == j) { c[x] = cj; s[x] = sj; }
     }
 }
 
@@ -132,64 +145,102 @@ __device__ __forceinline__ void add_bias(Row8& r, const Row8& b) {
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// x / scale to a code; scale 0 (a block of zeros) gives code 0.
+// A block's scale with what dividing by it takes.  Quotients are rounded as
+// the division itself would: q0 = x / scale by the rounded reciprocal, then
+// one correction by the exact remainder (Markstein's theorem: correctly
+// rounded when the reciprocal is).  Scale 0 (a block of zeros) gives 0; with a
+// scale that is not finite the remainder is NaN and q0 = x * 0 or NaN stands.
+struct Divisor {
+    float scale, inverse;
+    bool finite;
+    __device__ __forceinline__ explicit Divisor(float s) {
+        scale = s;
+        inverse = s == 0.f ? 0.f : __frcp_rn(s);
+        finite = abs_bits(s) < 0x7f800000u;
+    }
+    __device__ __forceinline__ float quotient(float x) const {
+        const float q0 = __fmul_rn(x, inverse);
+        const float q = __fmaf_rn(__fmaf_rn(-q0, scale, x), inverse, q0);
+        return copysignf(finite ? q : q0, x);       // a zero keeps its sign
+    }
+};
+
 template <class Code>
-__device__ __forceinline__ uint32_t code4(const float (&x)[4], float scale) {
+__device__ __forceinline__ uint32_t code4(const float (&x)[4], const Divisor& d) {
     float y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = scale == 0.f ? 0.f : __fdiv_rn(x[j], scale);
-    return Code::encode4(y[0], y[1], y[2], y[3]);
+    for (int j = 0; j < 4; ++j) y[j] = d.quotient(x[j]);
+    return Code::encode4(y, d.finite);
 }
 
 // One run: rows t .. t + n - 1 (n <= 16) of K or V head h go to rows row0 ..
-// of the block at `slot`.  The whole warp takes part.
+// of the block at `slot`.  The whole CTA takes part; tops: one word per warp.
 template <int D, class Code>
 __device__ __forceinline__ void append_run(const AppendParams& p, int which, int h, int t, int n,
-                                           long long slot, const Row8& bias, bool biased,
-                                           int lane) {
+                                           long long slot, const uint2 (&bias)[2], bool biased,
+                                           uint32_t* tops) {
     constexpr int LPR = D / 8;
-    constexpr int RPW = 32 / LPR;               // rows per pass
-    constexpr int PASSES = kKv8Block / RPW;
-    const int sub = lane / LPR, f0 = (lane % LPR) * 4;
+    constexpr int RPW = 32 / LPR;               // rows per warp and pass
+    constexpr int PASSES = kKv8Block / (RPW * kAppendWarps);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int sub = warp * RPW + lane / LPR, f0 = (lane % LPR) * 4;
+    constexpr int STEP = RPW * kAppendWarps;
     const Kv8View& c = p.cache;
-    const int page = int(slot / c.page_size), r0 = int(slot % c.page_size);
+    const int page = int(slot / c.page_size), r0 = int(slot - (long long)page * c.page_size);
     const int first = r0 % kKv8Block;           // rows of the block that are held already
-    const __half* x = (which ? p.v : p.k) + (size_t)h * D;
+    const __half* x = (which ? p.v : p.k) + (size_t)h * D + f0;
     __half* y = which ? p.v_out : p.k_out;
     const long long xs = p.stride[1 + which], ys = p.stride[4 + which];
     uint8_t* pool = which ? c.v : c.k;
     float* scale_at = reinterpret_cast<float*>(c.scale(page, h, r0)) + which;
-    const float old = first ? *scale_at : 0.f;
 
+    uint2 raw[PASSES][2];
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int j = i * STEP + sub;
+        if (j < n) {
+            const __half* src = x + (t + j) * xs;
+            raw[i][0] = *reinterpret_cast<const uint2*>(src);
+            raw[i][1] = *reinterpret_cast<const uint2*>(src + D / 2);
+        }
+    }
+    const float old = first ? *scale_at : 0.f;
     Row8 rows[PASSES];
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-        const int j = i * RPW + sub;
-        if (j < n) rows[i] = load_row<D>(x + (size_t)(t + j) * xs, f0);
-    }
-#pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        const int j = i * RPW + sub;
+        const int j = i * STEP + sub;
         if (j < n) {
-            if (biased) add_bias(rows[i], bias);
+            Row8& r = rows[i];
+            unpack4(raw[i][0], r.lo);
+            unpack4(raw[i][1], r.hi);
+            if (biased) {
+                Row8 b;
+                unpack4(bias[0], b.lo);
+                unpack4(bias[1], b.hi);
+                add_bias(r, b);
+            }
             if (!which) {
                 float cc[4], ss[4];
                 load_turn<D>(p, t + j, f0, cc, ss);
-                turn(rows[i], cc, ss);
+                turn(r, cc, ss);
             }
-            if (y) store_row<D>(y + (size_t)(t + j) * ys + (size_t)h * D, f0, rows[i]);
+            if (y) store_row<D>(y + (t + j) * ys + (size_t)h * D, f0, r);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                top = max(top, max(abs_bits(rows[i].lo[e]), abs_bits(rows[i].hi[e])));
+            for (int e = 0; e < 4; ++e) top = max(top, max(abs_bits(r.lo[e]), abs_bits(r.hi[e])));
         }
     }
     top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();                            // every warp has read the old scale, too
+#pragma unroll
+    for (int w = 0; w < kAppendWarps; ++w) top = max(top, tops[w]);
     float scale = __fdiv_rn(__uint_as_float(top), Code::kMax);
     if (first) scale = __uint_as_float(max(abs_bits(scale), abs_bits(old)));
+    const Divisor d(scale);
     if (first && abs_bits(scale) > abs_bits(old)) {
 #pragma unroll 1
-        for (int j = sub; j < first; j += RPW) {
+        for (int j = sub; j < first; j += STEP) {
             uint8_t* dst = pool + c.row(page, h, r0 - first + j);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -198,97 +249,115 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int which, int
                 float z[4];
 #pragma unroll
                 for (int b = 0; b < 4; ++b) z[b] = __fmul_rn(Code::decode(codes >> (8 * b)), old);
-                *w = code4<Code>(z, scale);
+                *w = code4<Code>(z, d);
             }
         }
     }
+    uint8_t* dst = pool + c.row(page, h, r0) + f0;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-        const int j = i * RPW + sub;
+        const int j = i * STEP + sub;
         if (j < n) {
-            uint8_t* dst = pool + c.row(page, h, r0 + j);
-            *reinterpret_cast<uint32_t*>(dst + f0) = code4<Code>(rows[i].lo, scale);
-            *reinterpret_cast<uint32_t*>(dst + f0 + D / 2) = code4<Code>(rows[i].hi, scale);
+            uint8_t* at = dst + j * c.row_stride;
+            *reinterpret_cast<uint32_t*>(at) = code4<Code>(rows[i].lo, d);
+            *reinterpret_cast<uint32_t*>(at + D / 2) = code4<Code>(rows[i].hi, d);
         }
     }
-    if (lane == 0) *scale_at = scale;
+    if (threadIdx.x == 0) *scale_at = scale;
+    __syncthreads();                            // the next run may be of this block; tops are reused
 }
 
-// Warps 0 .. kv_tasks - 1: (WINDOW tokens, K or V, kv head), doing the blocks
-// that one of these tokens is the first of; the warps after them: query rows, a lane group per (token, kQHeads heads).
-template <int D, int WINDOW, class Code>
-__global__ void __launch_bounds__(kAppendThreads)
+// CTAs 0 .. kv_ctas - 1: (p.window tokens, K or V, kv head), doing the blocks
+// that one of these tokens is the first of; the CTAs after them: query rows, a
+// lane group per (token, p.q_heads heads).  (Spreading the first among the
+// others measured the same or slower.)
+template <int D, class Code>
+__global__ void __launch_bounds__(kAppendThreads, 8)
 kv8_append_kernel(const __grid_constant__ AppendParams p) {
     constexpr int LPR = D / 8;
     constexpr int RPW = 32 / LPR;
+    __shared__ uint32_t tops[kAppendWarps];
     const int lane = threadIdx.x & 31;
-    const long long task = (long long)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
     const int Hkv = p.cache.Hkv;
-    const int windows = (p.T + WINDOW - 1) / WINDOW;
-    const long long kv_tasks = 2LL * windows * Hkv;
     const int f0 = (lane % LPR) * 4;
     grid_launch_dependents();
     grid_dependency_wait();
-    if (task < kv_tasks) {
-        const int h = int(task % Hkv);
-        const int which = int(task / Hkv) & 1;
-        const int t0 = int(task / (2 * Hkv)) * WINDOW;
+    if (blockIdx.x < p.kv_ctas) {
+        const int h = blockIdx.x % Hkv;
+        const int which = (blockIdx.x / Hkv) & 1;
+        const int t0 = blockIdx.x / (2 * Hkv) * p.window;
         const long long pool = (long long)p.cache.num_pages * p.cache.page_size;
-        // Lane l holds the slot of token t - 15 + l (lane 31 none): the tokens
-        // that can share a block with t.
-        long long slot[WINDOW];
-#pragma unroll
-        for (int w = 0; w < WINDOW; ++w) {
-            const int tl = t0 + w - 15 + lane;
-            slot[w] = tl >= 0 && tl < p.T && lane < 31 ? p.slots[tl] : -1;
-        }
         const __half* b = p.bias[1 + which];
-        Row8 bias = {};
-        if (b) bias = load_row<D>(b + (size_t)h * D, f0);
-#pragma unroll
-        for (int w = 0; w < WINDOW; ++w) {
-            const long long s = __shfl_sync(0xffffffffu, slot[w], 15);
-            if (s >= pool && lane == 15) record_error(p.err, kDevBadIndex);
-            if (s < 0 || s >= pool) continue;                       // uniform over the warp
-            const bool same = slot[w] >= 0 && slot[w] / kKv8Block == s / kKv8Block;
-            const uint32_t block = __ballot_sync(0xffffffffu, same);
-            if (block & 0x7fffu) continue;                          // an earlier token's warp has it
-            const long long before = __shfl_up_sync(0xffffffffu, slot[w], 1);
-            const uint32_t on = __ballot_sync(0xffffffffu, same && slot[w] == before + 1) >> 15;
-            uint32_t left = block >> 15;                            // bit j: token t + j
+        uint2 bias[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+        if (b) {
+            bias[0] = *reinterpret_cast<const uint2*>(b + (size_t)h * D + f0);
+            bias[1] = *reinterpret_cast<const uint2*>(b + (size_t)h * D + f0 + D / 2);
+        }
+        // Lane l holds the slot of token t - 15 + l: the tokens that can share
+        // a block with t (lane 31: the last token that can follow t + 15).
+        auto slots_about = [&](int t) {
+            const int tl = t - 15 + lane;
+            const long long s = tl >= 0 && tl < p.T ? p.slots[tl] : -1;
+            if (s >= pool) record_error(p.err, kDevBadIndex);
+            return s >= 0 && s < pool ? s : -1;
+        };
+        // The window's tokens (lanes 15 ..) that no earlier token shares a block with
+        const long long near = slots_about(t0);
+        const bool mine = lane >= 15 && lane < 15 + p.window;
+        const uint32_t mates = __match_any_sync(0xffffffffu, near >= 0 ? near / kKv8Block : -1LL);
+        uint32_t firsts = __ballot_sync(0xffffffffu, mine && near >= 0 && __ffs(mates) - 1 == lane);
+#pragma unroll 1
+        while (firsts) {                                            // uniform over the CTA
+            const int t = t0 + __ffs(firsts) - 16;
+            firsts &= firsts - 1;
+            const long long slot = t == t0 ? near : slots_about(t);
+            const long long s = __shfl_sync(0xffffffffu, slot, 15);
+            const bool same = lane >= 15 && lane < 31 && slot >= 0 && slot / kKv8Block == s / kKv8Block;
+            const long long before = __shfl_up_sync(0xffffffffu, slot, 1);
+            const uint32_t on = __ballot_sync(0xffffffffu, same && slot == before + 1) >> 15;
+            uint32_t left = __ballot_sync(0xffffffffu, same) >> 15; // bit j: token t + j
+#pragma unroll 1
             while (left) {
                 const int i = __ffs(left) - 1;
                 const int n = __ffs(~(on >> (i + 1)));              // 1 + the tokens that go on
                 left &= ~(((1u << n) - 1u) << i);
-                const long long si = __shfl_sync(0xffffffffu, slot[w], 15 + i);
-                append_run<D, Code>(p, which, h, t0 + w + i, n, si, bias, b != nullptr, lane);
-                __syncwarp();                                       // the next run of the block reads it
+                const long long si = __shfl_sync(0xffffffffu, slot, 15 + i);
+                append_run<D, Code>(p, which, h, t + i, n, si, bias, b != nullptr, tops);
             }
         }
         return;
     }
-    const int chunks = (p.H + kQHeads - 1) / kQHeads;
-    const long long item = (task - kv_tasks) * RPW + lane / LPR;
+    const int chunks = (p.H + p.q_heads - 1) / p.q_heads;
+    const long long item = ((long long)(blockIdx.x - p.kv_ctas) * kAppendWarps + (threadIdx.x >> 5)) * RPW + lane / LPR;
     if (item >= (long long)p.T * chunks) return;
     const int t = int(item / chunks);
-    const int h0 = int(item - (long long)t * chunks) * kQHeads;
-    const long long slot = p.slots[t];
-    if (slot < 0) return;
-    const __half* src = p.q + (size_t)t * p.stride[0];
-    __half* dst = p.q_out + (size_t)t * p.stride[3];
-    Row8 r[kQHeads];
-#pragma unroll
-    for (int j = 0; j < kQHeads; ++j)
-        if (h0 + j < p.H) r[j] = load_row<D>(src + (size_t)(h0 + j) * D, f0);
+    const int h_beg = int(item - (long long)t * chunks) * p.q_heads;
+    const int h_end = min(h_beg + p.q_heads, p.H);
+    if (p.slots[t] < 0) return;
+    const __half* src = p.q + t * p.stride[0] + f0;
+    __half* dst = p.q_out + t * p.stride[3];
     float c[4], s[4];
     load_turn<D>(p, t, f0, c, s);
+#pragma unroll 1
+    for (int h0 = h_beg; h0 < h_end; h0 += kQHeads) {
+        uint2 raw[kQHeads][2];
 #pragma unroll
-    for (int j = 0; j < kQHeads; ++j)
-        if (h0 + j < p.H) {
-            if (p.bias[0]) add_bias(r[j], load_row<D>(p.bias[0] + (size_t)(h0 + j) * D, f0));
-            turn(r[j], c, s);
-            store_row<D>(dst + (size_t)(h0 + j) * D, f0, r[j]);
-        }
+        for (int j = 0; j < kQHeads; ++j)
+            if (h0 + j < h_end) {
+                raw[j][0] = *reinterpret_cast<const uint2*>(src + (h0 + j) * D);
+                raw[j][1] = *reinterpret_cast<const uint2*>(src + (h0 + j) * D + D / 2);
+            }
+#pragma unroll
+        for (int j = 0; j < kQHeads; ++j)
+            if (h0 + j < h_end) {
+                Row8 r;
+                unpack4(raw[j][0], r.lo);
+                unpack4(raw[j][1], r.hi);
+                if (p.bias[0]) add_bias(r, load_row<D>(p.bias[0] + (size_t)(h0 + j) * D, f0));
+                turn(r, c, s);
+                store_row<D>(dst + (size_t)(h0 + j) * D, f0, r);
+            }
+    }
 }
 
 // ---------------------------------------------------------------------------

@@ -35,7 +35,7 @@ struct Kv8View {
 
 // Code types.  half2_lo / half2_hi widen the low / high two bytes of a word
 // to fp16 exactly (both types' values are fp16 numbers); encode4 rounds four
-// scaled values to the nearest codes, ties to even, saturating.
+// values, already divided by their scale, to the nearest codes, ties to even.
 struct Int8Code {
     static constexpr float kMax = 127.f;
     static constexpr bool kHasNan = false;
@@ -56,12 +56,15 @@ struct Int8Code {
     static __device__ __forceinline__ float decode(uint32_t byte) {
         return float(int8_t(byte & 0xff));
     }
-    static __device__ __forceinline__ uint32_t encode(float x) {
-        // NaN (in a block whose scale is not finite) converts to 0; the scale carries it
-        return uint32_t(max(-127, min(127, __float2int_rn(x)))) & 0xffu;
-    }
-    static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
-        return encode(a) | (encode(b) << 8) | (encode(c) << 16) | (encode(d) << 24);
+    // x + 1.5 * 2^23 is rounded to an integer (ties to even), whose low byte is
+    // the code; |x| <= 127.  A block whose scale is not finite has codes 0: the
+    // scale carries it.
+    static __device__ __forceinline__ uint32_t encode4(const float (&x)[4], bool finite) {
+        uint32_t b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(__fadd_rn(x[i], 12582912.f));
+        const uint32_t lo = __byte_perm(b[0], b[1], 0x0040), hi = __byte_perm(b[2], b[3], 0x0040);
+        return finite ? __byte_perm(lo, hi, 0x5410) : 0u;
     }
 };
 
@@ -89,8 +92,8 @@ struct E4m3Code {
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
         return r;
     }
-    static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
-        return encode2(a, b) | (encode2(c, d) << 16);
+    static __device__ __forceinline__ uint32_t encode4(const float (&x)[4], bool) {
+        return encode2(x[0], x[1]) | (encode2(x[2], x[3]) << 16);
     }
 };
 
