@@ -266,16 +266,19 @@ int fr_paged_step(const int* kv_lens, const int* new_lens, int* block_table, int
         fr::StepParams p{kv_lens, new_lens, block_table, free_pages, free_count, kv_lens_out,
                          free_count_out, token_offsets, positions, slots, status, nullptr, batch,
                          page_size, num_pages, max_blocks_per_seq, max_tokens};
-        // One CTA per 1024 tokens, at most one per SM; several share a counter
-        // of the workspace.  A capture without a workspace runs with one CTA.
-        int ctas = std::min(st->sm_count, (max_tokens + fr::kStepThreads - 1) / fr::kStepThreads);
-        if (ctas > 1) {
+        // One CTA per 1024 tokens or 256 requests (whose pages change hands),
+        // at most one per SM.  Several that update the lengths in place share a
+        // counter of the workspace; a capture without a workspace runs with one.
+        int ctas = std::min(st->sm_count, std::max((max_tokens + fr::kStepThreads - 1) / fr::kStepThreads,
+                                                   (batch + 255) / 256));
+        if (ctas > 1 && (kv_lens_out == kv_lens || free_count_out == free_count)) {
             rc = ensure_workspace(st, kCounterBytes, s);
             if (rc == FR_ERR_WORKSPACE) ctas = 1;
             else if (rc != FR_OK) return rc;
             else p.ticket = static_cast<int*>(st->ws);
         }
-        return launch_plain(fr::paged_step_kernel, (unsigned)ctas, fr::kStepThreads, smem, s,
+        const unsigned threads = ctas == 1 && batch <= 256 ? 256 : fr::kStepThreads;
+        return launch_plain(fr::paged_step_kernel, (unsigned)ctas, threads, smem, s,
                             static_cast<const fr::StepParams>(p));
     });
 }

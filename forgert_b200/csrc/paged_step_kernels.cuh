@@ -13,8 +13,8 @@
 // Every CTA forms the three prefix sums in shared memory (the lengths are a
 // few KB, read from L2) and takes its share of the tokens and pages; a token
 // finds its request by binary search.  kv_lens_out may be kv_lens and
-// free_count_out free_count: they are written by the CTA that is last to have
-// read the inputs (one counter, zero between calls), so no CTA waits.
+// free_count_out free_count: they are then written by the CTA that is last to
+// have read the inputs (one counter, zero between calls), so no CTA waits.
 //
 // What bounds it: latency (a launch, two dependent rounds of loads, the scan)
 // for a decode step; 12 bytes written per token for long prompts.
@@ -47,7 +47,7 @@ struct StepParams {
     int* positions;
     long long* slots;
     int* status;
-    int* ticket;           // nullptr with one CTA
+    int* ticket;           // nullptr: one CTA, or no output over its input
     int batch, page_size, num_pages, max_blocks, max_tokens;
 };
 
@@ -142,38 +142,11 @@ paged_step_kernel(const StepParams p) {
     else if (toks > p.max_tokens) status = kStepTooMany;
     else if (take > count + give) status = kStepNoPages;
 
-    // Every input of this CTA's in-place outputs is read: the last CTA to come
-    // here writes them.
-    if (tid == 0) {
-        int last = 1;
-        if (p.ticket) last = atom_add_acq_rel_gpu(p.ticket, 1) == (int)gridDim.x - 1;
-        last_cta = last;
-        if (last && p.ticket) *p.ticket = 0;
-    }
-    __syncthreads();
-    if (last_cta) {
-        // new_lens is only read by the call: ended or grown requests are told by the prefix sums
-        for (int b = tid; b < B; b += blockDim.x) {
-            int after;
-            if (status != kStepOk) after = p.kv_lens[b];
-            else if (p.new_lens[b] < 0) after = 0;
-            else after = kv[b] + ftok[b + 1] - ftok[b];
-            p.kv_lens_out[b] = after;
-        }
-        if (tid == 0) {
-            *p.free_count_out = status == kStepOk ? count + give - take : count;
-            *p.status = status;
-        }
-    }
+    // This CTA has read every input of the in-place outputs.  The count is only
+    // looked at after the tokens, when it has long come back.
+    int arrived = 0;
+    if (tid == 0 && p.ticket) arrived = atom_add_acq_rel_gpu(p.ticket, 1);
     const int stride = gridDim.x * blockDim.x, at = blockIdx.x * blockDim.x + tid;
-    if (status != kStepOk) {                    // nothing changes: no token has a place
-        for (int b = at; b <= B; b += stride) p.token_offsets[b] = 0;
-        for (int t = at; t < p.max_tokens; t += stride) {
-            p.positions[t] = 0;
-            p.slots[t] = -1;
-        }
-        return;
-    }
     auto released = [&](int i) {                // i-th released page
         const int b = last_at_most(fgive, B, i);
         return p.block_table[(size_t)b * p.max_blocks + (i - fgive[b])];
@@ -181,18 +154,24 @@ paged_step_kernel(const StepParams p) {
     auto popped = [&](int i) {
         return i < give ? released(give - 1 - i) : p.free_pages[count - 1 - (i - give)];
     };
-    for (int b = at; b <= B; b += stride) p.token_offsets[b] = ftok[b];
-    // Entries read above (of released rows, of the stack below count) and
-    // written below (of growing rows, of the stack from count up) are distinct.
-    for (int i = at; i < give; i += stride) p.free_pages[count + i] = released(i);
-    for (int i = at; i < take; i += stride) {
-        const int b = last_at_most(ftake, B, i);
-        p.block_table[(size_t)b * p.max_blocks + (kv[b] + P - 1) / P + (i - ftake[b])] = popped(i);
-    }
+    const bool go = status == kStepOk;          // a refused step changes nothing: no token has a place
+    auto finish = [&](int first, int step) {    // lengths and the stack's height after the step
+        for (int b = first; b < B; b += step) {
+            int after = p.kv_lens[b];           // refused: as it was, fitting or not
+            if (go) after = p.new_lens[b] < 0 ? 0 : kv[b] + ftok[b + 1] - ftok[b];
+            p.kv_lens_out[b] = after;
+        }
+        if (first == 0) {
+            *p.free_count_out = go ? count + give - take : count;
+            *p.status = status;
+        }
+    };
+    if (!p.ticket) finish(at, stride);
+    for (int b = at; b <= B; b += stride) p.token_offsets[b] = go ? ftok[b] : 0;
     for (int t = at; t < p.max_tokens; t += stride) {
         int pos = 0;
         long long slot = -1;
-        if (t < toks) {
+        if (go && t < toks) {
             const int b = last_at_most(ftok, B, t);
             pos = kv[b] + (t - ftok[b]);
             const int idx = pos / P, have = (kv[b] + P - 1) / P;
@@ -203,6 +182,23 @@ paged_step_kernel(const StepParams p) {
         p.positions[t] = pos;
         p.slots[t] = slot;
     }
+    if (go) {
+        // Entries read (of released rows, of the stack below count) and written
+        // (of growing rows, of the stack from count up) are distinct.
+        for (int i = at; i < give; i += stride) p.free_pages[count + i] = released(i);
+        for (int i = at; i < take; i += stride) {
+            const int b = last_at_most(ftake, B, i);
+            p.block_table[(size_t)b * p.max_blocks + (kv[b] + P - 1) / P + (i - ftake[b])] = popped(i);
+        }
+    }
+    // In place: the CTA that was last to have read the inputs writes them.
+    if (!p.ticket) return;
+    if (tid == 0) {
+        last_cta = arrived == (int)gridDim.x - 1;
+        if (last_cta) *p.ticket = 0;
+    }
+    __syncthreads();
+    if (last_cta) finish(tid, blockDim.x);
 }
 
 }  // namespace fr
