@@ -62,7 +62,7 @@ struct DeviceState {
     int persist_occ[4] = {0};    // CTAs/SM of the persistent batched kernels
     int resident[4][5] = {{-1, -1, -1, -1, -1}, {-1, -1, -1, -1, -1}, {-1, -1, -1, -1, -1},
                           {-1, -1, -1, -1, -1}};   // co-resident clusters per (slot, log2 size)
-    int kv8_occ[8] = {0};        // CTAs/SM of the 8-bit decode kernels (0 = not prepared)
+    int kv8_occ[16] = {0};       // CTAs/SM of the 8-bit decode kernels (0 = not prepared)
     bool step_ready = false;     // paged_step_kernel's shared-memory attribute set
     int resident_g[4][2] = {{-1, -1}, {-1, -1}, {-1, -1}, {-1, -1}};   // grouped form, 8 / 16
 };

@@ -43,54 +43,60 @@ fr::Kv8View kv8_view(const fr_kv8_cache* c) {
     return v;
 }
 
-// Shape of the decode kernel: four warps, steps of 16 (D = 128) or 32 (D = 64)
-// rows, 4 KB of codes.  Up to 8 query heads per kv head: four CTAs per SM (128
-// registers) and two steps under way per warp; more: three CTAs (168 registers,
-// the second 8-head tile's state spills at 128) and three steps.
+// Shapes of the decode kernel: four warps, steps of 16 (D = 128) or 32 (D = 64)
+// rows, 4 KB of codes.
+//   for long calls, as many warps as an SM holds: up to 8 query heads per kv
+//     head four CTAs (128 registers) with two steps under way per warp, more
+//     three CTAs (168 registers: the second 8-head tile's state spills at 128)
+//     with three;
+//   DEEP, for calls of few tiles per SM, where warps are few anyway and wait
+//     for memory: fewer CTAs with more steps under way.
+template <int NT, bool DEEP> struct Kv8Shape;
+template <> struct Kv8Shape<1, false> { static constexpr int kCtas = 4, kStages = 2; };
+template <> struct Kv8Shape<2, false> { static constexpr int kCtas = 3, kStages = 3; };
+template <> struct Kv8Shape<1, true> { static constexpr int kCtas = 3, kStages = 4; };
+template <> struct Kv8Shape<2, true> { static constexpr int kCtas = 2, kStages = 6; };
 constexpr int kKv8Warps = 4;
-template <int NT> constexpr int kv8_ctas() { return NT == 1 ? 4 : 3; }
-template <int NT> constexpr int kv8_stages() { return NT == 1 ? 2 : 3; }
 template <int D> constexpr int kv8_mt() { return 128 / D; }
 constexpr int kv8_tile(int head_dim) { return 16 * (128 / head_dim) * kKv8Warps; }
 
-template <int D, int NT>
-using Kv8SmemOf = fr::Kv8Smem<D, NT, kv8_mt<D>(), kv8_stages<NT>(), kKv8Warps>;
+template <int D, int NT, bool DEEP>
+using Kv8SmemOf = fr::Kv8Smem<D, NT, kv8_mt<D>(), Kv8Shape<NT, DEEP>::kStages, kKv8Warps>;
 
-template <int D, int NT, class Code>
+template <int D, int NT, bool DEEP, class Code>
 auto kv8_ptr() {
-    return fr::kv8_decode_kernel<D, NT, kv8_mt<D>(), kv8_stages<NT>(), kKv8Warps, kv8_ctas<NT>(),
-                                 Code>;
+    using Shape = Kv8Shape<NT, DEEP>;
+    return fr::kv8_decode_kernel<D, NT, kv8_mt<D>(), Shape::kStages, kKv8Warps, Shape::kCtas, Code>;
 }
 
-template <int D, int NT, class Code>
+template <int D, int NT, bool DEEP, class Code>
 int prepare_kv8(DeviceState* st, int slot) {
     std::lock_guard<std::mutex> lk(g_prep_mu);
     if (st->kv8_occ[slot]) return FR_OK;
-    const int bytes = static_cast<int>(Kv8SmemOf<D, NT>::kBytes);
-    cudaError_t e = cudaFuncSetAttribute(kv8_ptr<D, NT, Code>(),
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const int bytes = static_cast<int>(Kv8SmemOf<D, NT, DEEP>::kBytes);
+    auto fn = kv8_ptr<D, NT, DEEP, Code>();
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return cuda_fail(e);
     int n = 0;
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv8_ptr<D, NT, Code>(),
-                                                      32 * kKv8Warps, bytes);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, 32 * kKv8Warps, bytes);
     if (e != cudaSuccess) return cuda_fail(e);
     st->kv8_occ[slot] = std::max(1, n);
     return FR_OK;
 }
 
-template <int D, int NT, class Code>
+template <int D, int NT, bool DEEP, class Code>
 int launch_kv8(const fr::Kv8DecodeParams& kp, int ctas, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, 1, 1);
     cfg.blockDim = dim3(32 * kKv8Warps, 1, 1);
-    cfg.dynamicSmemBytes = Kv8SmemOf<D, NT>::kBytes;
+    cfg.dynamicSmemBytes = Kv8SmemOf<D, NT, DEEP>::kBytes;
     cfg.stream = s;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_ptr<D, NT, Code>(), kp);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_ptr<D, NT, DEEP, Code>(), kp);
     g_launches.fetch_add(1, std::memory_order_relaxed);
     if (e == cudaSuccess) e = cudaGetLastError();
     return e == cudaSuccess ? FR_OK : cuda_fail(e);
@@ -127,6 +133,7 @@ int kv8_chunk(int batch, int num_kv_heads, int head_groups, int head_dim, int ma
 
 struct Kv8Plan {
     int nt = 1, head_groups = 1, chunk = 0, ctas = 0;
+    bool deep = false;
     size_t ws_bytes = 0;
 };
 
@@ -138,14 +145,21 @@ int kv8_plan(DeviceState* st, int batch, int num_heads, int num_kv_heads, int he
     pl.head_groups = (group + 8 * pl.nt - 1) / (8 * pl.nt);
     pl.chunk = kv8_chunk(batch, num_kv_heads, pl.head_groups, head_dim, max_kv_len);
     if (pl.chunk <= 0) return FR_ERR_INVALID_ARG;
-    const int slot = (head_dim == 64 ? 0 : 4) + (pl.nt - 1) * 2 + dtype;
-    int rc = kv8_dispatch(head_dim, pl.nt, dtype, [&](auto d, auto n, auto code) {
-        return prepare_kv8<decltype(d)::value, decltype(n)::value, decltype(code)>(st, slot);
-    });
-    if (rc != FR_OK) return rc;
     const int tile = kv8_tile(head_dim);
     const long long tiles = (long long)pl.chunk * num_kv_heads * pl.head_groups *
                             std::max(1, (max_kv_len + tile - 1) / tile);
+    // The deep shape up to 22 tiles per SM, were every sequence as long as the
+    // longest may be (28 / 4 heads of 128, deep / long shape: one sequence of
+    // 4096 tokens 11.5 / 14.3 us, 64 of up to 300 10.1 / 12.3, 24 of up to 2000
+    // 14.0 / 16.4, 48 of up to 1300 19.4 / 18.2, 64 of up to 8192 57.9 / 49.9).
+    pl.deep = tiles <= 22LL * st->sm_count;
+    const int slot = (head_dim == 64 ? 0 : 8) + (pl.nt - 1) * 4 + (pl.deep ? 2 : 0) + dtype;
+    int rc = kv8_dispatch(head_dim, pl.nt, dtype, [&](auto d, auto n, auto code) {
+        constexpr int D = decltype(d)::value, NT = decltype(n)::value;
+        return pl.deep ? prepare_kv8<D, NT, true, decltype(code)>(st, slot)
+                       : prepare_kv8<D, NT, false, decltype(code)>(st, slot);
+    });
+    if (rc != FR_OK) return rc;
     pl.ctas = (int)std::max<long long>(
         1, std::min<long long>((long long)st->sm_count * st->kv8_occ[slot], tiles));
     pl.ws_bytes = kCounterBytes + (size_t)2 * pl.ctas * 8 * pl.nt * (head_dim + 2) * sizeof(float);
@@ -180,14 +194,17 @@ int run_kv8(const void* q, long long q_stride, const fr_kv8_cache* cache, const 
     p.max_units = kKv8Units;
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(st->ws) + kCounterBytes);
     p.part_acc = p.part_ml + (size_t)2 * pl.ctas * 8 * pl.nt * 2;
-    // At least four tiles per CTA before SMs get more than one; a unit's start
+    // At least two tiles per CTA before SMs get more than one.  A unit's start
     // and its merge are charged as one tile each (four each, which suits the
     // 16-bit kernel's longer tiles, left too few CTAs to short calls: one
-    // sequence of 2048 tokens 18.6 us instead of 10.6).
-    p.min_tiles_per_cta = 4;
+    // sequence of 2048 tokens 18.6 us instead of 10.6), and units of up to six
+    // tiles are not cut: 64 sequences of 200 to 300 tokens 17.4 -> 12.4 us, no
+    // call measured slower.
+    p.min_tiles_per_cta = 2;
     p.min_ctas = st->sm_count;
     p.item_cost = 1;
     p.merge_cost = 1;
+    p.whole_tiles = 6;
     for (int b = 0; b < batch; b += pl.chunk) {
         p.batch = std::min(pl.chunk, batch - b);
         p.q = static_cast<const __half*>(q) + (size_t)b * q_stride;
@@ -195,7 +212,9 @@ int run_kv8(const void* q, long long q_stride, const fr_kv8_cache* cache, const 
         p.kv_lens = kv_lens + b;
         p.block_table = block_table + (size_t)b * max_blocks;
         rc = kv8_dispatch(D, pl.nt, cache->dtype, [&](auto d, auto n, auto code) {
-            return launch_kv8<decltype(d)::value, decltype(n)::value, decltype(code)>(p, pl.ctas, s);
+            constexpr int kD = decltype(d)::value, NT = decltype(n)::value;
+            return pl.deep ? launch_kv8<kD, NT, true, decltype(code)>(p, pl.ctas, s)
+                           : launch_kv8<kD, NT, false, decltype(code)>(p, pl.ctas, s);
         });
         if (rc != FR_OK) return rc;
     }

@@ -56,16 +56,20 @@ struct Kv8DecodeParams {
     int max_len;                 // lengths are cut to this
     int min_tiles_per_cta, min_ctas;
     int item_cost, merge_cost;   // in tile times, see ShareMap
+    int whole_tiles;             // at least 1, see ShareMap
     float scale_log2;            // log2(e) / sqrt(D)
 };
 
 // Cost-balanced shares in 32-bit arithmetic.  A unit of nb tiles spans xc + nb
 // + mc cost points: xc before its first tile (starting an item), mc after its
 // last (merging).  Of Ctot points CTA c takes the c-th of C equal shares (the
-// first Ctot mod C one point longer) and the tiles whose points lie in it.
+// first Ctot mod C one point longer) and the tiles whose points lie in it; a
+// border that falls into a short unit moves to the unit's nearer end, since
+// cutting it costs a merge (some CTAs are then left without tiles).
 struct ShareMap {
     const int* seq_start;        // tiles before each sequence, all units
     int B, upb, xc, mc;
+    int whole;                   // units of at most this many tiles are not cut
     int C, share, extra;         // Ctot = C * share + extra
 
     __device__ __forceinline__ void split(int Ctot, int ctas) {
@@ -86,7 +90,8 @@ struct ShareMap {
         const int span = nb + xc + mc;
         const int off = v - cs(lo);
         const int j = min(off / span, upb - 1);
-        const int i = max(0, min(off - j * span - xc, nb - 1));
+        int i = max(0, min(off - j * span - xc, nb - 1));
+        if (nb <= whole) i = 2 * i <= nb ? 0 : nb;      // to the unit's nearer end
         return seq_start[lo] + j * nb + i;
     }
     // CTA that holds tile i of unit j of sequence b: the one with the tile's
@@ -604,15 +609,18 @@ kv8_decode_kernel(const __grid_constant__ Kv8DecodeParams p) {
     scan_lengths<TILE>(p.kv_lens, B, upb, seq_start, lens, warp_sums, p.max_len);
 
     const int T = seq_start[B];
-    ShareMap sm{seq_start, B, upb, p.item_cost, p.merge_cost, 0, 0, 0};
+    ShareMap sm{seq_start, B, upb, p.item_cost, p.merge_cost, p.whole_tiles, 0, 0, 0};
     const int Ctot = T + B * upb * (sm.xc + sm.mc);
     int C = min((int)gridDim.x, T);
     if (p.min_tiles_per_cta > 0) C = min(C, max(p.min_ctas, T / p.min_tiles_per_cta));
-    sm.split(Ctot, max(1, min(C, Ctot / (sm.xc + sm.mc + 2))));
+    // No tile of a unit that may be cut spans as many points as a share has, so
+    // every CTA from a cut unit's first to its last holds a piece of it.
+    sm.split(Ctot, max(1, min(C, Ctot / (max(sm.xc, sm.mc) + 1))));
     if (blockIdx.x >= sm.C) return;
     const int beg = sm.beg(blockIdx.x);
     const int end = sm.beg(blockIdx.x + 1);
     const int n = end - beg;
+    if (n == 0) return;                         // its share lies within a unit that another took whole
 
     TileCursor cur;
     cur.seek(seq_start, B, upb, beg);
