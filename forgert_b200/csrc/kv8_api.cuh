@@ -337,6 +337,10 @@ int fr_qkv_rope_append_kv8(const void* q, const void* k, const void* v, void* q_
         if (used && p.stride[i] < heads[i] * D) return FR_ERR_INVALID_ARG;
         if (used && (p.stride[i] & 3)) return FR_ERR_MISALIGNED;
     }
+    // An output over its input has to lie as the input does.
+    if ((q_out == q && p.stride[3] != p.stride[0]) || (k_out == k && p.stride[4] != p.stride[1]) ||
+        (v_out == v && p.stride[5] != p.stride[2]))
+        return FR_ERR_INVALID_ARG;
     for (const void* a : {q, k, v, (const void*)q_out, (const void*)k_out, (const void*)v_out,
                           q_bias, k_bias, v_bias, (const void*)slots})
         if (!aligned(a, 8)) return FR_ERR_MISALIGNED;

@@ -374,10 +374,12 @@ __device__ __forceinline__ void consume_kv8(uint32_t kst, uint32_t vst, const fl
                     xp = fmaxf(xp, __shfl_xor_sync(0xffffffffu, xp, d));
                     xw = fmaxf(xw, __shfl_xor_sync(0xffffffffu, xw, d));
                 }
-                // exponents are relative to the reference (0 while there is none), kShift up
+                // Exponents are relative to the reference (0 while there is none),
+                // kShift up.  A column moves for its own terms only: no head's
+                // bits depend on another's.
                 const float m0 = st.m[nt][j], w0 = st.mv[nt][j];
-                const float m1 = fmaxf(m0, (m0 == -INFINITY ? 0.f : m0) - kShift + xp);
-                const float w1 = fmaxf(w0, (w0 == -INFINITY ? 0.f : w0) - kShift + xw);
+                const float m1 = m0 == -INFINITY ? xp - kShift : xp > kTop ? m0 - kShift + xp : m0;
+                const float w1 = w0 == -INFINITY ? xw - kShift : xw > kTop ? w0 - kShift + xw : w0;
                 const float fl = m0 == -INFINITY ? 0.f : fast_exp2(m0 - m1);
                 const float fo = w0 == -INFINITY ? 0.f : fast_exp2(w0 - w1);
                 st.m[nt][j] = m1;

@@ -260,7 +260,8 @@ FR_API int fr_prefill_attn(const void* q, const void* k, const void* v, void* ou
  * so token-major pages or K and V interleaved in one allocation work too.
  * One K and one V scale belong to each block of FR_KV8_BLOCK consecutive rows
  * of a page and each kv head:
- *   scales [num_pages][num_kv_heads][page_size / FR_KV8_BLOCK][2] fp32 (K, V)
+ *   scales [num_pages][num_kv_heads][page_size / FR_KV8_BLOCK][2] fp32 (K, V),
+ *          not negative
  * Slot s is row s % page_size of page s / page_size. */
 #define FR_KV8_INT8 0          /* codes -127 .. 127 */
 #define FR_KV8_E4M3 1          /* 4 exponent, 3 mantissa bits; largest 448 */
@@ -320,7 +321,8 @@ FR_API int fr_paged_step(const int* kv_lens, const int* new_lens, int* block_tab
  *   q_out       may be q; k_out, v_out: NULL (decode: only the cache is
  *               needed) or a buffer, which may be k, v (prefill attention)
  *   token_strides  host array of 6: halves between consecutive tokens of q,
- *               k, v, q_out, k_out, v_out (multiples of 4); NULL = contiguous
+ *               k, v, q_out, k_out, v_out (multiples of 4; an output in place
+ *               has its input's); NULL = contiguous
  *   *_bias      fp16 [heads * head_dim] or NULL
  *   cos_tab, sin_tab  [table_rows, head_dim / 2] fp32 (fr_rope_tables)
  *   positions   int32 [num_axes, num_tokens]; frequency f turns by table row

@@ -169,3 +169,14 @@ def test_handle_checks():
             A.KV8Cache(*args)
     with pytest.raises(ValueError, match="CUDA"):
         A.KV8Cache(k, k, s)
+
+
+def test_append_in_place_keeps_the_layout(lib):
+    """An output over its input with another distance between tokens would be
+    written where other tokens are still read."""
+    c = cache()
+    inv = _lib.FR_ERR_INVALID_ARG
+    assert append(lib, c, strides=[512, 128, 128, 516, 128, 128], qo=FAKE) == inv
+    assert append(lib, c, strides=[512, 128, 128, 512, 132, 128], ko=FAKE) == inv
+    assert append(lib, c, strides=[512, 128, 128, 512, 128, 136], vo=FAKE) == inv
+    assert append(lib, c, strides=[512, 128, 128, 516, 132, 136], qo=FAKE + 64, ko=FAKE + 64, vo=FAKE + 64, T=0) == _lib.FR_OK

@@ -335,3 +335,103 @@ def test_refusals():
         A.decode_attn_paged_kv8(q.data_ptr() + 8, cache, t, n, q, 2, 8, 2, 64)
     with pytest.raises(ValueError):
         A.decode_attn_paged_kv8(q.cpu(), cache, t, n, q, 2, 8, 2, 64)
+
+
+# ------------------------------------------------- the shape for long calls
+# A call whose bound max_kv_len allows many tiles runs another shape of the
+# kernel; the lengths themselves may be short.  With int8 codes and up to 8
+# heads it takes q in 16-bit fixed point on the head's largest value: an
+# element is off by 1 / 65278 of that, a score by at most
+# max|q| sum |k_i| / (65278 sqrt(D)), which the bound doubles as it does the
+# rounding of the scores' sums.
+
+def run_long(q, cache, table, lens, page_size):
+    bound = (1 << 19) // page_size * page_size
+    wide = np.full((len(lens), bound // page_size), -1, np.int32)
+    wide[:, :table.shape[1]] = table
+    return run(q, cache, wide, lens, max_kv_len=bound)
+
+
+def check_long(got, q, kc, vc, scales, code, table, lens):
+    k = O.values(kc, scales, 0, code)
+    r, mass, big = O.attention(q, k, O.values(vc, scales, 1, code), table, lens)
+    B, H, D = q.shape
+    fixed = np.zeros_like(big)
+    for b, n in enumerate(lens):
+        ids = np.asarray(table[b][:-(-max(0, n) // kc.shape[2])], np.int64)
+        for j in range(kc.shape[1]):
+            rows = np.abs(k[ids, j]).sum(-1).reshape(-1)[:max(0, n)]
+            g = H // kc.shape[1]
+            if len(rows):
+                fixed[b, j * g:(j + 1) * g, 0] = rows.max() * np.abs(q[b, j * g:(j + 1) * g].astype(np.float64)).max(-1)
+    fixed /= 65278 * np.sqrt(D)
+    tol = 2.0 ** -11 * np.abs(r) + (2.0 ** -11 + 2.0 ** -13 + 2 * D * 2.0 ** -23 * big + 2 * fixed) * mass + 1e-7
+    err = np.abs(got.astype(np.float64) - r)
+    assert np.isfinite(got).all()
+    assert (err <= tol).all(), f"max err / tol {(err / tol).max():.3f}"
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("H,Hkv,D", SHAPES + [(24, 2, 64), (9, 1, 64), (33, 1, 128)])
+def test_long_shape(H, Hkv, D, code):
+    rng = np.random.default_rng(H + D)
+    lens = [0, 1, 15, 16, 17, 129, 700, 4097, 0, 2049, 20000]
+    q = half(rng, (len(lens), H, D))
+    table, pages = make_table(rng, lens, 48)
+    kc, vc, scales = make_pool(rng, pages, Hkv, 48, D, code)
+    poison(table, lens, 48, (kc, vc), scales, code)
+    cache = to_cache(kc, vc, scales, code)
+    got = run_long(q, cache, table, lens, 48)
+    assert (got[[0, 8]] == 0).all()
+    check_long(got, q, kc, vc, scales, code, table, lens)
+    for _ in range(3):
+        assert np.array_equal(run_long(q, cache, table, lens, 48), got)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_query_extremes(D, long, code):
+    """Heads of zeros, of the smallest and of large halves, of one large
+    element; NaN and infinity spoil their own head only."""
+    rng = np.random.default_rng(D)
+    lens = [333, 40]
+    q = half(rng, (2, 7, D))
+    q[0, 0] = 0
+    q[0, 1] = np.float16(6e-8)
+    q[0, 2] *= np.float16(300)
+    q[0, 3, 1:] = 0
+    q[1, 4] = np.float16(-2.0)
+    table, pages = make_table(rng, lens, 32)
+    kc, vc, scales = make_pool(rng, pages, 1, 32, D, code)
+    cache = to_cache(kc, vc, scales, code)
+
+    def call(x):
+        return run_long(x, cache, table, lens, 32) if long else run(x, cache, table, lens)
+
+    clean = call(q)
+    check_long(clean, q, kc, vc, scales, code, table, lens)
+    bad = q.copy()
+    bad[0, 5, 3], bad[1, 6, 0] = np.nan, np.inf
+    got = call(bad)
+    assert np.isnan(got[0, 5]).all() and np.isnan(got[1, 6]).all()
+    keep = np.ones((2, 7), bool)
+    keep[0, 5] = keep[1, 6] = False
+    assert np.array_equal(got[keep], clean[keep])
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_long_shape_wide_scales_and_zero_blocks(code):
+    """Blocks whose scales differ by many powers of two, blocks of zero scale."""
+    rng = np.random.default_rng(21)
+    lens = [900, 31, 64]
+    q = half(rng, (3, 28, 128))
+    table, pages = make_table(rng, lens, 32)
+    kc, vc, scales = make_pool(rng, pages, 4, 32, 128, code)
+    scales[..., 1] *= np.exp2(rng.integers(-30, 6, scales.shape[:3])).astype(np.float32)
+    scales[..., 0] *= np.exp2(rng.integers(-6, 2, scales.shape[:3])).astype(np.float32)
+    scales[table[0, 3], :, 0] = 0.0
+    scales[table[2, :2], 1, :, 1] = 0.0           # a whole sequence's V of one kv head
+    got = run_long(q, to_cache(kc, vc, scales, code), table, lens, 32)
+    check_long(got, q, kc, vc, scales, code, table, lens)
+    assert (got[2, 7:14] == 0).all()
