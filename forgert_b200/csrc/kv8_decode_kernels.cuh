@@ -12,7 +12,10 @@
 // its bits.  The row sum uses the unrounded probabilities.
 //
 // Bound: HBM.  2 * D bytes of codes per position and kv head, plus 8 bytes of
-// scales per 16 positions; 4 * D * G operations on them.
+// scales per 16 positions; 4 * D * G operations on them.  Measured, 28 / 4
+// heads of 128: 64 sequences of 8192 to 32768 tokens in e4m3 204 us, 6.4 TB/s
+// (0.98 of a copy's rate); of 1024 to 8192 50 us, 5.4 TB/s, of which about 7
+// are launch, first rows, fold and merge; one sequence of 512 tokens 8.
 //
 // Decomposition: persistent CTAs take equal shares of the batch's work, as in
 // batched_kernels.cuh (units, items, pieces merged by the contributor that

@@ -16,8 +16,9 @@
 // free_count_out free_count: they are then written by the CTA that is last to
 // have read the inputs (one counter, zero between calls), so no CTA waits.
 //
-// What bounds it: latency (a launch, two dependent rounds of loads, the scan)
-// for a decode step; 12 bytes written per token for long prompts.
+// What bounds it: latency (a launch, two dependent rounds of loads, the scan, a
+// search per token): 64 requests 3.5 us in a graph, 1024 requests with 122
+// thousand new tokens 8.9 (0.2 us of bytes).
 #pragma once
 #include "fr_ptx.cuh"
 #include <cstdint>
