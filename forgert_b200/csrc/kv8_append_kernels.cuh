@@ -22,10 +22,10 @@
 // of cosines and sines.  The four warps of a CTA share a run's 16 rows, which
 // stay in registers (two rows' eighths a lane) from the load to the codes.
 // (One warp per run, 64 values a lane: 128 registers and straight-line code
-// that the instruction cache lost, 60 us for 4600 tokens of 28 / 4 heads.)
+// that the instruction cache lost, 60 us for 4800 tokens of 28 / 4 heads.)
 //
 // Bound: for prompts issue slots (63 % of the cycles) and the loads' latency at
-// 27 warps per SM - 4600 tokens of 28 / 4 heads of 128, three axes, biases and
+// 27 warps per SM - 4800 tokens of 28 / 4 heads of 128, three axes, biases and
 // 16-bit K and V written too, 24 us, 4.0 TB/s; for a decode step latency, four
 // dependent rounds of loads (64 tokens 7 us).
 #pragma once
@@ -147,6 +147,8 @@ __device__ __forceinline__ void add_bias(Row8& r, const Row8& b) {
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
+constexpr float kMinScale = 0x1p-100f;  // of a block that is not zeros
+
 // A block's scale with what dividing by it takes.  Quotients are rounded as
 // the division itself would: q0 = x / scale by the rounded reciprocal, then
 // one correction by the exact remainder (Markstein's theorem: correctly
@@ -239,6 +241,8 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int which, int
     for (int w = 0; w < kAppendWarps; ++w) top = max(top, tops[w]);
     float scale = __fdiv_rn(__uint_as_float(top), Code::kMax);
     if (first) scale = __uint_as_float(max(abs_bits(scale), abs_bits(old)));
+    // A smaller one's reciprocal and remainders would leave fp32's range.
+    if (abs_bits(scale) - 1u < abs_bits(kMinScale) - 1u) scale = kMinScale;
     const Divisor d(scale);
     if (first && abs_bits(scale) > abs_bits(old)) {
 #pragma unroll 1

@@ -107,6 +107,8 @@ def put(rows, codes, scales, which, slots, code):
                 scale = np.float32(top / kmax)
                 if first:
                     scale = np.float32(np.nan) if np.isnan(scale) or np.isnan(old) else max(scale, np.abs(old))
+                if 0 < scale < np.float32(2.0 ** -100):
+                    scale = np.float32(2.0 ** -100)
                 grew = first and not np.isnan(old) and (np.isnan(scale) or scale > abs(old))
                 if grew:
                     held = codes[page, h, r0 - first:r0]

@@ -333,3 +333,25 @@ def test_refusals():
     with pytest.raises(ForgeRTError, match="invalid argument"):
         A.kv8_gather(pool.cache, slots, None, None, 2)
     pool.same()
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_tiny_values(code):
+    """Rotated values far below what fp16 holds: a scale stops at 2^-100, above
+    it the codes are those of the division, remainders included."""
+    rng = np.random.default_rng(11)
+    for size in (1e-18, 1e-24, 1e-27, 1e-29, 1e-38):
+        pool = Pool(rng, 4, 2, 16, 64, code)
+        pool.scales[:] = 0
+        pool.sd.zero_()
+        T = 16
+        slots, pos = np.arange(T, dtype=np.int64) + 16, np.arange(T, dtype=np.int32)[None]
+        q, k, v = half(rng, (T, 4, 64)), half(rng, (T, 2, 64)), half(rng, (T, 2, 64))
+        cos, sin = (x * np.float32(size) for x in tables(64))
+        with np.errstate(under="ignore"):
+            O.append(q, k, v, [None] * 3, cos, sin, pos, [0] * 32, slots, pool.k, pool.v, pool.scales, code)
+        A.qkv_rope_append_kv8(dev(q), dev(k), dev(v), dev(q), None, None, dev(cos), dev(sin), dev(pos), dev(slots),
+                              pool.cache, T, 4, ROWS)
+        torch.cuda.synchronize()
+        pool.same()
+        assert pool.scales[1, 0, 0, 0] >= 2.0 ** -100
