@@ -334,10 +334,10 @@ FR_API int fr_paged_step(const int* kv_lens, const int* new_lens, int* block_tab
  * Scales: consecutive tokens of a call in consecutive rows of one block are
  * coded together with scale amax / (127 or 448), at least the block's old
  * scale if they do not start at its row 0 (the rows below them are then taken
- * to be held); if the scale grows, those rows are coded anew.  A scale is 0 (a block of zeros) or at
- * least 2^-100.  A call's tokens
- * of one block lie within 16 consecutive tokens, as fr_paged_step lays them
- * out, and are taken in token order.  A block that holds a NaN or an infinity reads back as NaN.
+ * to be held); if the scale grows, those rows are coded anew.  A scale is 0 (a
+ * block of zeros) or at least 2^-100.  A call's tokens of one block lie within
+ * 16 consecutive tokens, as fr_paged_step lays them out, and are taken in
+ * token order.  A block that holds a NaN or an infinity reads back as NaN.
  * A position outside the table (read as 0) or a slot outside the pool (not
  * cached) is recorded: fr_get_device_error then gives device code 4 and
  * FR_ERR_INVALID_ARG.  num_tokens 0 does nothing. */
