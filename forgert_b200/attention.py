@@ -207,6 +207,7 @@ class KV8Cache:
             raise ValueError("scales must be contiguous fp32 "
                              "[num_pages, num_kv_heads, page_size / 16, 2]")
         self.k, self.v, self.scales = k, v, scales
+        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = pages, heads, rows, dim
         strides = [k.stride(i) for i in range(3)]
         # a dimension of one element never steps: give it a stride the checks accept
         strides = [s if n > 1 else max(s, -(-dim // 16) * 16) // 16 * 16
@@ -257,7 +258,7 @@ def qkv_rope_append_kv8(q, k, v, q_out, k_out, v_out, cos_tab, sin_tab, position
     cache is wanted) and every output its input; token_strides: halves between
     tokens of q, k, v, q_out, k_out, v_out."""
     lib = load()
-    if freq_axis is not None and len(freq_axis) != cache._struct.head_dim // 2:
+    if freq_axis is not None and len(freq_axis) != cache.head_dim // 2:
         raise ValueError("freq_axis must name an axis for each of the head_dim / 2 frequencies")
     strides = None
     if token_strides is not None:

@@ -293,6 +293,13 @@ kv8_append_kernel(const __grid_constant__ AppendParams p) {
         const int which = (blockIdx.x / Hkv) & 1;
         const int t0 = blockIdx.x / (2 * Hkv) * p.window;
         const long long pool = (long long)p.cache.num_pages * p.cache.page_size;
+        // The window's rows are on their way to L2 while the slots are read.
+        {
+            const int tr = t0 + threadIdx.x / (D / 64);             // 128 bytes each
+            if (threadIdx.x < p.window * (D / 64) && tr < p.T)
+                prefetch_l2((which ? p.v : p.k) + tr * p.stride[1 + which] + (size_t)h * D +
+                            threadIdx.x % (D / 64) * 64);
+        }
         const __half* b = p.bias[1 + which];
         uint2 bias[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
         if (b) {
@@ -339,20 +346,27 @@ kv8_append_kernel(const __grid_constant__ AppendParams p) {
     const int t = int(item / chunks);
     const int h_beg = int(item - (long long)t * chunks) * p.q_heads;
     const int h_end = min(h_beg + p.q_heads, p.H);
-    if (p.slots[t] < 0) return;
     const __half* src = p.q + t * p.stride[0] + f0;
     __half* dst = p.q_out + t * p.stride[3];
-    float c[4], s[4];
-    load_turn<D>(p, t, f0, c, s);
-#pragma unroll 1
-    for (int h0 = h_beg; h0 < h_end; h0 += kQHeads) {
-        uint2 raw[kQHeads][2];
+    // The first rows and the angles are on their way before the slot tells
+    // whether the token takes part.
+    const long long slot = p.slots[t];
+    uint2 raw[kQHeads][2];
+    auto load_heads = [&](int h0) {
 #pragma unroll
         for (int j = 0; j < kQHeads; ++j)
             if (h0 + j < h_end) {
                 raw[j][0] = *reinterpret_cast<const uint2*>(src + (h0 + j) * D);
                 raw[j][1] = *reinterpret_cast<const uint2*>(src + (h0 + j) * D + D / 2);
             }
+    };
+    load_heads(h_beg);
+    if (slot < 0) return;
+    float c[4], s[4];
+    load_turn<D>(p, t, f0, c, s);
+#pragma unroll 1
+    for (int h0 = h_beg; h0 < h_end; h0 += kQHeads) {
+        if (h0 > h_beg) load_heads(h0);
 #pragma unroll
         for (int j = 0; j < kQHeads; ++j)
             if (h0 + j < h_end) {
