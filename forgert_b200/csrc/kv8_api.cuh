@@ -48,9 +48,7 @@ fr::Kv8View kv8_view(const fr_kv8_cache* c) {
 //   for long calls, as many warps as an SM holds: up to 8 query heads per kv
 //     head four CTAs (128 registers) with two steps under way per warp, more
 //     three CTAs (168 registers: the second 8-head tile's state spills at 128)
-//     with three; up to 8 heads of int8 take q in integer planes (64 sequences
-//     of 8192 to 32768 tokens 220.6 -> 210.4 us; a short call's first scores
-//     come 1.1 us later, and two 8-head tiles spill);
+//     with three;
 //   DEEP, for calls of few tiles per SM, where warps are few anyway and wait
 //     for memory: fewer CTAs with more steps under way.
 template <int NT, bool DEEP> struct Kv8Shape;
@@ -68,8 +66,7 @@ using Kv8SmemOf = fr::Kv8Smem<D, NT, kv8_mt<D>(), Kv8Shape<NT, DEEP>::kStages, k
 template <int D, int NT, bool DEEP, class Code>
 auto kv8_ptr() {
     using Shape = Kv8Shape<NT, DEEP>;
-    return fr::kv8_decode_kernel<D, NT, kv8_mt<D>(), Shape::kStages, kKv8Warps, Shape::kCtas,
-                                 Code::kPlanes && !DEEP && NT == 1, Code>;
+    return fr::kv8_decode_kernel<D, NT, kv8_mt<D>(), Shape::kStages, kKv8Warps, Shape::kCtas, Code>;
 }
 
 template <int D, int NT, bool DEEP, class Code>

@@ -39,7 +39,6 @@ struct Kv8View {
 struct Int8Code {
     static constexpr float kMax = 127.f;
     static constexpr bool kHasNan = false;
-    static constexpr bool kPlanes = true;       // codes can enter an integer product as they are
     // With the sign bit flipped a code is u = code + 128 in 0..255, and the
     // fp16 with bits 0x6400 | u is 1024 + u: subtracting 1152 is exact.
     static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w ^ 0x80808080u; }
@@ -72,7 +71,6 @@ struct Int8Code {
 struct E4m3Code {
     static constexpr float kMax = 448.f;
     static constexpr bool kHasNan = true;       // codes 0x7f and 0xff
-    static constexpr bool kPlanes = false;
     static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w; }
     static __device__ __forceinline__ uint32_t widen16(uint16_t x) {
         uint32_t h;

@@ -195,14 +195,13 @@ struct Kv8State {
 };
 
 // q of one item as the B operand, in the order that K's words come in: lane
-// (g, t) holds dims (D/4) * t .. of head g.  As fp16 pairs; or (PLANES, int8
-// codes) in 16-bit fixed point on the head's largest value, as two s8 planes
-// (x = 256 hi + lo), whose products with the codes are exact: an element is
-// off by 2^-17 of the largest at most.  unit[j]: that of head column 2t + j.
-template <int D, int NT, bool PLANES>
+// (g, t) holds dims (D/4) * t .. of head g, as fp16 pairs.  (int8 codes can
+// also enter integer products, with q in 16-bit fixed point on its head's
+// largest value as two s8 planes: 64 sequences of 8192 to 32768 tokens 210 us
+// instead of 221, but a channel far above the others takes their bits.)
+template <int D, int NT>
 struct Kv8Query {
     uint32_t b[D / 16][NT][2];
-    float unit[NT][2];
 
     __device__ __forceinline__ void load(const __half* q, int gcount, int lane) {
         const int g = lane >> 2, t = lane & 3;
@@ -217,48 +216,15 @@ struct Kv8Query {
                 b[w][nt][0] = v.x; b[w][nt][1] = v.y;
                 b[w + 1][nt][0] = v.z; b[w + 1][nt][1] = v.w;
             }
-            unit[nt][0] = unit[nt][1] = 1.f;
-            if (PLANES) to_planes(nt, t);
-        }
-    }
-    __device__ __forceinline__ void to_planes(int nt, int t) {
-        uint32_t top = 0;                       // largest |q| by its bits: NaN above all
-#pragma unroll
-        for (int w = 0; w < D / 16; ++w)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                top = max(top, max(b[w][nt][e] & 0x7fffu, (b[w][nt][e] >> 16) & 0x7fffu));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float big = __half2float(__ushort_as_half((unsigned short)top));
-        const bool usable = top < 0x7c00u && top > 0;
-        const float inv = usable ? 32639.f / big : 0.f;         // 127 * 256 + 127
-        // not finite: every score of the head is NaN
-        const float mine = top < 0x7c00u ? big * (1.f / 32639.f) : __int_as_float(0x7fffffff);
-        unit[nt][0] = __shfl_sync(0xffffffffu, mine, (2 * t) * 4);
-        unit[nt][1] = __shfl_sync(0xffffffffu, mine, (2 * t + 1) * 4);
-#pragma unroll
-        for (int w = 0; w < D / 16; ++w) {      // four dims: a word of each plane
-            uint32_t v[4], h[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t x = b[w][nt][e >> 1] >> (16 * (e & 1));
-                const float f = usable ? __half2float(__ushort_as_half((unsigned short)x)) : 0.f;
-                v[e] = __float_as_uint(fmaf(f, inv, 12582912.f));       // 0x4b400000 + integer
-                h[e] = v[e] + 128u;                                     // byte 1: (x + 128) >> 8
-            }
-            // bytes 0 are x - 256 hi, as s8
-            b[w][nt][0] = __byte_perm(__byte_perm(h[0], h[1], 0x0051), __byte_perm(h[2], h[3], 0x0051), 0x5410);
-            b[w][nt][1] = __byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410);
         }
     }
 };
 
 // One step: 16 * MT rows of K at kst and V at vst, of which the first `valid`
 // (>= 1) are positions; sc: their blocks' scales.
-template <int D, int NT, int MT, bool PLANES, class Code>
+template <int D, int NT, int MT, class Code>
 __device__ __forceinline__ void consume_kv8(uint32_t kst, uint32_t vst, const float2* sc, int valid,
-                                            const Kv8Query<D, NT, PLANES>& q,
+                                            const Kv8Query<D, NT>& q,
                                             Kv8State<D, NT>& st, float sl2, int lane) {
     constexpr int KL = D / 64;                  // 16-byte loads per K row and lane
     constexpr int VW = D / 32;                  // words per V row and lane
@@ -281,17 +247,10 @@ __device__ __forceinline__ void consume_kv8(uint32_t kst, uint32_t vst, const fl
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         const int r = mt * 16 + rg;
-        // Planes: sums below 2^22 counted up from the bits of 1.5 * 2^23, so
-        // that as floats they are that number plus the sum, exactly.
-        constexpr int kBias = 0x4b400000;
-        int hi[NT][4], lo[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                s[mt][nt][c] = 0.f;
-                hi[nt][c] = lo[nt][c] = kBias;
-            }
+            for (int c = 0; c < 4; ++c) s[mt][nt][c] = 0.f;
 #pragma unroll
         for (int j = 0; j < KL; ++j) {
             const int chunk = KL * t + j;
@@ -301,30 +260,13 @@ __device__ __forceinline__ void consume_kv8(uint32_t kst, uint32_t vst, const fl
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const int ks0 = j * 4 + w;
-                if constexpr (PLANES) {
-                    if (w % 2) continue;        // two words are one k-step of 32
+                const uint32_t xw = Code::prepare(xs[w]), yw = Code::prepare(ys[w]);
+                const uint32_t a0 = Code::half2_lo(xw), a1 = Code::half2_lo(yw);
+                const uint32_t a2 = Code::half2_hi(xw), a3 = Code::half2_hi(yw);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma_16832_s8(hi[nt], xs[w], ys[w], xs[w + 1], ys[w + 1], q.b[ks0][nt][0], q.b[ks0 + 1][nt][0]);
-                        mma_16832_s8(lo[nt], xs[w], ys[w], xs[w + 1], ys[w + 1], q.b[ks0][nt][1], q.b[ks0 + 1][nt][1]);
-                    }
-                } else {
-                    const uint32_t xw = Code::prepare(xs[w]), yw = Code::prepare(ys[w]);
-                    const uint32_t a0 = Code::half2_lo(xw), a1 = Code::half2_lo(yw);
-                    const uint32_t a2 = Code::half2_hi(xw), a3 = Code::half2_hi(yw);
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        mma_16816(s[mt][nt], a0, a1, a2, a3, q.b[ks0][nt][0], q.b[ks0][nt][1]);
-                }
+                for (int nt = 0; nt < NT; ++nt)
+                    mma_16816(s[mt][nt], a0, a1, a2, a3, q.b[ks0][nt][0], q.b[ks0][nt][1]);
             }
-        }
-        if constexpr (PLANES) {
-            const float bias = __int_as_float(kBias);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    s[mt][nt][c] = fmaf(__int_as_float(hi[nt][c]) - bias, 256.f, __int_as_float(lo[nt][c]) - bias);
         }
     }
 
@@ -344,9 +286,8 @@ __device__ __forceinline__ void consume_kv8(uint32_t kst, uint32_t vst, const fl
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int c = j; c < 4; c += 2) {
-                        const float f = PLANES ? ks[mt] * q.unit[nt][j] : ks[mt];
-                        ep[mt][nt][c] = fmaf(s[mt][nt][c], f, -mp);
-                        ew[mt][nt][c] = fmaf(s[mt][nt][c], f, lv[mt] - mw);
+                        ep[mt][nt][c] = fmaf(s[mt][nt][c], ks[mt], -mp);
+                        ew[mt][nt][c] = fmaf(s[mt][nt][c], ks[mt], lv[mt] - mw);
                         if (tail && mt * 16 + rg + (c >> 1) * 8 >= valid)
                             ep[mt][nt][c] = ew[mt][nt][c] = -INFINITY;
                         top = fmaxf(top, fmaxf(ep[mt][nt][c], ew[mt][nt][c]));
@@ -672,7 +613,7 @@ __device__ __forceinline__ void kv8_merge(const Kv8DecodeParams& p, float* area,
 // Persistent kernel: grid = C co-resident CTAs of NW warps; see
 // persistent_decode_kernel for units, items, pieces and the merge.
 // ---------------------------------------------------------------------------
-template <int D, int NT, int MT, int STAGES, int NW, int CTAS, bool PLANES, class Code>
+template <int D, int NT, int MT, int STAGES, int NW, int CTAS, class Code>
 __global__ void __launch_bounds__(32 * NW, CTAS)
 kv8_decode_kernel(const __grid_constant__ Kv8DecodeParams p) {
     constexpr int TILE = 16 * MT * NW;
@@ -771,7 +712,7 @@ kv8_decode_kernel(const __grid_constant__ Kv8DecodeParams p) {
         const int len = lens[b];
         const size_t head_base = (size_t)b * p.H + h0;
 
-        Kv8Query<D, NT, PLANES> q;
+        Kv8Query<D, NT> q;
         q.load(p.q + (size_t)b * p.q_stride + (size_t)h0 * D, gcount, lane);
         Kv8State<D, NT> st;
         st.clear();
@@ -783,8 +724,8 @@ kv8_decode_kernel(const __grid_constant__ Kv8DecodeParams p) {
             const uint32_t kst = ring + stage * (2 * S::kStepBytes);
             const int valid = len - ((i0 + tt) * NW + warp) * (16 * MT);
             if (valid > 0)
-                consume_kv8<D, NT, MT, PLANES, Code>(kst, kst + S::kStepBytes, scales + stage * MT, valid, q,
-                                             st, sl2, lane);
+                consume_kv8<D, NT, MT, Code>(kst, kst + S::kStepBytes, scales + stage * MT, valid, q, st,
+                                             sl2, lane);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
         cur.advance(seq_start, B, upb, cnt);
