@@ -4,7 +4,8 @@ server calls them.
 Requests come with prompts of different lengths, are decoded token by token,
 end, and others start in their rows:
 
-  paged_step              pages, positions and slots of the step's tokens
+  paged_step              pages, positions and slots of the step's tokens,
+                          packed in request order
   per layer
     qkv_rope_append_kv8   bias + RoPE, K/V coded into the layer's cache
     prefill_attn_causal   prompts, on the 16-bit K/V that the append returns
@@ -27,7 +28,12 @@ import math
 
 class Server:
     """`rows` request slots over one pool of pages (shared by all layers, each
-    with a cache of its own)."""
+    with a cache of its own).
+
+    A step's tokens are packed: token t of the step is row t of prefill's q, k
+    and v.  decode's have one row per request instead, whether it takes part
+    or not.
+    """
 
     def __init__(self, rows: int, num_heads: int, num_kv_heads: int, head_dim: int, layers: int,
                  page_size: int, num_pages: int, max_len: int, max_tokens: int, dtype,
@@ -47,9 +53,13 @@ class Server:
         self.free_pages = torch.arange(num_pages, **i32)
         self.free_count = torch.full((1,), num_pages, **i32)
         self.offsets = torch.zeros(rows + 1, **i32)
-        self.positions = torch.zeros(max_tokens, **i32)
-        self.slots = torch.full((max_tokens,), -1, dtype=torch.int64, device="cuda")
+        # one entry more than a step writes: of a request without a token
+        self.positions = torch.zeros(max_tokens + 1, **i32)
+        self.slots = torch.full((max_tokens + 1,), -1, dtype=torch.int64, device="cuda")
         self.status = torch.zeros(1, **i32)
+        # of each request's first token of the step; slot -1 without one
+        self.row_positions = torch.zeros(rows, **i32)
+        self.row_slots = torch.full((rows,), -1, dtype=torch.int64, device="cuda")
         self.cos, self.sin = A.rope_tables_device(rope_rows, head_dim, theta)
         self.caches = [A.KV8Cache.empty(num_pages, page_size, num_kv_heads, head_dim, dtype)
                        for _ in range(layers)]
@@ -58,26 +68,38 @@ class Server:
 
     def step(self, max_tokens: int, stream=None) -> None:
         """Pages, positions and slots for new_lens, lengths moved on in place."""
+        import torch
+
         from . import attention as A
 
         A.paged_step(self.kv_lens, self.new_lens, self.table, self.free_pages, self.free_count,
                      self.kv_lens, self.free_count, self.offsets, self.positions, self.slots,
                      self.status, self.rows, self.page_size, self.num_pages, self.width,
                      max_tokens, stream=stream)
+        with torch.cuda.stream(torch.cuda.default_stream() if stream is None else stream):
+            first = self.offsets[:-1]
+            at = torch.where(self.offsets[1:] > first, first, self.max_tokens)
+            torch.index_select(self.positions, 0, at, out=self.row_positions)
+            torch.index_select(self.slots, 0, at, out=self.row_slots)
 
-    def append(self, layer: int, q, k, v, q_out, k_out, v_out, tokens: int, stream=None) -> None:
+    def append(self, layer: int, q, k, v, q_out, k_out, v_out, tokens: int, stream=None,
+               positions=None, slots=None) -> None:
+        """`tokens` rows at `positions` and `slots`, by default the packed tokens'."""
         from . import attention as A
 
-        A.qkv_rope_append_kv8(q, k, v, q_out, k_out, v_out, self.cos, self.sin, self.positions,
-                              self.slots, self.caches[layer], tokens, self.H, self.rope_rows,
-                              stream=stream)
+        A.qkv_rope_append_kv8(q, k, v, q_out, k_out, v_out, self.cos, self.sin,
+                              self.positions if positions is None else positions,
+                              self.slots if slots is None else slots, self.caches[layer], tokens,
+                              self.H, self.rope_rows, stream=stream)
 
     def decode(self, layer: int, q, k, v, out, stream=None) -> None:
-        """One layer of a decode step: rows tokens, one per request (a request
-        that takes no part has no slot, and its output means nothing)."""
+        """One layer of a step in which every request gets one token or none:
+        row b of q, k, v and out is request b's (a request that takes no part
+        has no slot: nothing of it is turned or cached, and its output means
+        nothing)."""
         from . import attention as A
 
-        self.append(layer, q, k, v, q, None, None, self.rows, stream)
+        self.append(layer, q, k, v, q, None, None, self.rows, stream, self.row_positions, self.row_slots)
         A.decode_attn_paged_kv8(q, self.caches[layer], self.table, self.kv_lens, out, self.rows,
                                 self.H, self.width, self.max_len, stream=stream)
 
@@ -87,9 +109,8 @@ class Server:
 
         from . import attention as A
 
-        tokens = len(q)
         k16, v16 = torch.empty_like(k), torch.empty_like(v)
-        self.append(layer, q, k, v, q, k16, v16, tokens)
+        self.append(layer, q, k, v, q, k16, v16, len(q))
         outs, at = [], 0
         for n in lens:
             out = torch.empty_like(q[at:at + n])
@@ -145,6 +166,7 @@ def run(requests: int = 16, layers: int = 4, steps: int = 64, code: str = "int8"
         s.new_lens.copy_(new)
         tokens = sum(lens.values())
         s.step(tokens)
+        assert int(s.status) == 0, f"step refused: {int(s.status)}"
         for layer in range(layers):
             s.prefill(layer, rand(tokens, num_heads, head_dim), rand(tokens, num_kv_heads, head_dim),
                       rand(tokens, num_kv_heads, head_dim), [lens[r] for r in sorted(lens)])

@@ -358,7 +358,9 @@ FR_API int fr_kv8_gather(const fr_kv8_cache* cache, const long long* slots, void
 
 /* Decode attention over the 8-bit paged cache, one token per sequence.
  *   q            [batch, num_heads, head_dim] fp16, q_stride halves between
- *                sequences (a multiple of 8; 0 = num_heads * head_dim), 16-byte aligned
+ *                sequences (a multiple of 8; 0 = num_heads * head_dim), 16-byte aligned.
+ *                Row b is sequence b's token: of the tokens that fr_paged_step
+ *                packs in request order, its newest is number token_offsets[b + 1] - 1
  *   out          [batch, num_heads, head_dim] fp16, 16-byte aligned
  *   block_table  device int32 [batch, max_blocks_per_seq]; page ids outside
  *                the pool read as zero rows
