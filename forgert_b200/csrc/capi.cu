@@ -57,6 +57,7 @@ struct DeviceState {
     int* err = nullptr;          // device error word
     void* ws = nullptr;          // split partial states
     size_t ws_bytes = 0;
+    std::vector<std::pair<void*, size_t>> old_ws;   // outgrown workspaces and their bytes
     uint32_t attr_done = 0;      // bit per kernel instantiation: smem attribute set
     int occupancy[8] = {0};      // CTAs/SM per instantiation (0 = not queried)
     int persist_occ[4] = {0};    // CTAs/SM of the persistent batched kernels
@@ -96,24 +97,31 @@ bool is_capturing(cudaStream_t s) {
     return cs != cudaStreamCaptureStatusNone;
 }
 
+// An outgrown workspace is kept: graphs captured with it go on using it.  Each
+// is larger than the one before it by a quarter at least, so the kept ones
+// together are smaller than four times the newest.
 int ensure_workspace(DeviceState* st, size_t bytes, cudaStream_t s) {
     if (bytes <= st->ws_bytes) return FR_OK;
     if (is_capturing(s)) return FR_ERR_WORKSPACE;
     std::lock_guard<std::mutex> lk(g_mu);
     if (bytes <= st->ws_bytes) return FR_OK;
-    if (st->ws) {
-        cudaError_t e = cudaDeviceSynchronize();
-        if (e != cudaSuccess) return cuda_fail(e);
-        cudaFree(st->ws);
-        st->ws = nullptr;
-        st->ws_bytes = 0;
+    try {
+        st->old_ws.reserve(st->old_ws.size() + 1);
+    } catch (...) {
+        return cuda_fail(cudaErrorMemoryAllocation);
     }
     const size_t grow = bytes + bytes / 4;
-    cudaError_t e = cudaMalloc(&st->ws, grow);
-    if (e != cudaSuccess) { st->ws = nullptr; return cuda_fail(e); }
-    // The fused merge's counters (start of the buffer) must be zero between calls.
-    e = cudaMemset(st->ws, 0, std::min(grow, kCounterBytes));
+    void* ws = nullptr;
+    cudaError_t e = cudaMalloc(&ws, grow);
     if (e != cudaSuccess) return cuda_fail(e);
+    // The fused merge's counters (start of the buffer) must be zero between calls.
+    e = cudaMemset(ws, 0, std::min(grow, kCounterBytes));
+    if (e != cudaSuccess) {
+        cudaFree(ws);
+        return cuda_fail(e);
+    }
+    if (st->ws) st->old_ws.push_back({st->ws, st->ws_bytes});
+    st->ws = ws;
     st->ws_bytes = grow;
     return FR_OK;
 }
@@ -1406,9 +1414,15 @@ int fr_get_device_error(int clear, int* device_code) {
             if (e != cudaSuccess) return cuda_fail(e);
         }
     }
-    if (clear && code && st && st->ws) {
+    if (clear && code && st) {
         // an aborted call may have left fused-merge counters behind
-        e = cudaMemset(st->ws, 0, std::min(st->ws_bytes, kCounterBytes));
+        std::lock_guard<std::mutex> lk(g_mu);
+        auto clear_counters = [](void* ws, size_t bytes) {
+            return ws ? cudaMemset(ws, 0, std::min(bytes, kCounterBytes)) : cudaSuccess;
+        };
+        e = clear_counters(st->ws, st->ws_bytes);
+        for (const auto& w : st->old_ws)
+            if (e == cudaSuccess) e = clear_counters(w.first, w.second);
         if (e != cudaSuccess) return cuda_fail(e);
     }
     if (device_code) *device_code = code;
@@ -1422,7 +1436,9 @@ size_t fr_allocated_bytes(void) {
     std::lock_guard<std::mutex> lk(g_mu);
     auto it = g_dev.find(dev);
     if (it == g_dev.end() || !it->second.err) return 0;
-    return sizeof(int) + it->second.ws_bytes;
+    size_t bytes = sizeof(int) + it->second.ws_bytes;
+    for (const auto& w : it->second.old_ws) bytes += w.second;
+    return bytes;
 }
 
 int fr_last_cuda_error(void) { return t_last_cuda; }

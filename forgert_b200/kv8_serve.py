@@ -63,8 +63,11 @@ class Server:
         self.cos, self.sin = A.rope_tables_device(rope_rows, head_dim, theta)
         self.caches = [A.KV8Cache.empty(num_pages, page_size, num_kv_heads, head_dim, dtype)
                        for _ in range(layers)]
-        # before any capture: the attention's partial states, the step's counter
-        A.reserve_workspace(A.kv8_workspace_size(rows, num_heads, num_kv_heads, head_dim, max_len))
+        # before any capture, once for good: the attention's partial states, the
+        # step's counter, and what a prompt of any length splits into
+        A.reserve_workspace(max(
+            A.kv8_workspace_size(rows, num_heads, num_kv_heads, head_dim, max_len),
+            max(A.prefill_workspace_size(n, num_heads, head_dim) for n in range(1, max_len + 1))))
 
     def step(self, max_tokens: int, stream=None) -> None:
         """Pages, positions and slots for new_lens, lengths moved on in place."""

@@ -21,7 +21,9 @@
  * few-head prompts) keep per-split (m, l, acc) partial states in a
  * library-owned per-device buffer that grows on demand with cudaMalloc.  Growth cannot happen inside CUDA-graph capture, so size it with
  * fr_reserve_workspace() before capturing; a capture that would need more
- * returns FR_ERR_WORKSPACE.  The buffer is shared by all calls on a device:
+ * returns FR_ERR_WORKSPACE.  A buffer that is outgrown is kept for the graphs
+ * captured with it (all kept ones are smaller together than four times the
+ * newest).  The buffer is shared by all calls on a device:
  * calls on different streams of one device must not overlap in time.
  */
 #ifndef FORGERT_ATTN_H
@@ -400,7 +402,7 @@ FR_API size_t fr_prefill_workspace_size(int seq_len, int num_heads, int head_dim
 FR_API int fr_get_device_error(int clear, int* device_code);
 
 /* Device memory the library has allocated with cudaMalloc on the current
- * device (its error word and workspace; exchange buffers are the caller's),
+ * device (its error word and workspaces; exchange buffers are the caller's),
  * 0 when none.  Creates no state and allocates nothing.  Diagnostics; no
  * reference counterpart. */
 FR_API size_t fr_allocated_bytes(void);
