@@ -71,6 +71,14 @@ struct DeviceState {
 std::mutex g_mu;
 std::unordered_map<int, DeviceState> g_dev;
 
+// Zeros device memory before it returns.  cudaMemset alone does not: it runs
+// on the default stream, perhaps after the call, and a non-blocking stream's
+// kernels would not wait for it.
+cudaError_t zero_now(void* p, size_t bytes) {
+    cudaError_t e = cudaMemset(p, 0, bytes);
+    return e == cudaSuccess ? cudaStreamSynchronize(nullptr) : e;
+}
+
 // Returns the current device's state, creating it (cudaMalloc of the error
 // word) on first use.  First use must therefore happen outside graph capture.
 int get_state(DeviceState** out) {
@@ -84,8 +92,12 @@ int get_state(DeviceState** out) {
         if (e != cudaSuccess) return cuda_fail(e);
         e = cudaMalloc(&st.err, sizeof(int));
         if (e != cudaSuccess) { st.err = nullptr; return cuda_fail(e); }
-        e = cudaMemset(st.err, 0, sizeof(int));
-        if (e != cudaSuccess) return cuda_fail(e);
+        e = zero_now(st.err, sizeof(int));
+        if (e != cudaSuccess) {
+            cudaFree(st.err);
+            st.err = nullptr;
+            return cuda_fail(e);
+        }
     }
     *out = &st;
     return FR_OK;
@@ -115,7 +127,7 @@ int ensure_workspace(DeviceState* st, size_t bytes, cudaStream_t s) {
     cudaError_t e = cudaMalloc(&ws, grow);
     if (e != cudaSuccess) return cuda_fail(e);
     // The fused merge's counters (start of the buffer) must be zero between calls.
-    e = cudaMemset(ws, 0, std::min(grow, kCounterBytes));
+    e = zero_now(ws, std::min(grow, kCounterBytes));
     if (e != cudaSuccess) {
         cudaFree(ws);
         return cuda_fail(e);
@@ -1410,7 +1422,7 @@ int fr_get_device_error(int clear, int* device_code) {
         if (e != cudaSuccess) return cuda_fail(e);
         if (!code) code = c;
         if (clear && c) {
-            e = cudaMemset(w, 0, sizeof(int));
+            e = zero_now(w, sizeof(int));
             if (e != cudaSuccess) return cuda_fail(e);
         }
     }
@@ -1418,7 +1430,7 @@ int fr_get_device_error(int clear, int* device_code) {
         // an aborted call may have left fused-merge counters behind
         std::lock_guard<std::mutex> lk(g_mu);
         auto clear_counters = [](void* ws, size_t bytes) {
-            return ws ? cudaMemset(ws, 0, std::min(bytes, kCounterBytes)) : cudaSuccess;
+            return ws ? zero_now(ws, std::min(bytes, kCounterBytes)) : cudaSuccess;
         };
         e = clear_counters(st->ws, st->ws_bytes);
         for (const auto& w : st->old_ws)

@@ -113,3 +113,37 @@ def test_serving_reserves_for_every_prompt():
     assert set(r["sizes"]) == {r["reserved"]}
     assert r["error"] == 0 and r["status"] == 0
     assert r["max_error"] <= 4 * (2.0 ** -11 + 2.0 ** -11) + 2.0 ** -10
+
+
+FIRST_CALL = r"""
+import json, torch
+from forgert_b200 import attention as A
+from oracle import kv8 as O
+B, ps, width, pages, max_tokens = 1025, 16, 8, 6000, 20000
+i32 = dict(dtype=torch.int32, device="cuda")
+new = [(b * 7) % 19 for b in range(B)]
+kv, newd = torch.zeros(B, **i32), torch.tensor(new, **i32)
+table, stack, count = torch.full((B, width), -1, **i32), torch.arange(pages, **i32), torch.tensor([pages], **i32)
+offsets, positions = torch.full((B + 1,), -7, **i32), torch.full((max_tokens,), -7, **i32)
+slots, status = torch.full((max_tokens,), -7, dtype=torch.int64, device="cuda"), torch.full((1,), -7, **i32)
+dirty = [torch.full((1 << 19,), -1, **i32) for _ in range(64)]
+torch.cuda.synchronize()
+del dirty
+torch.cuda.empty_cache()                    # what cudaMalloc gives next may hold ones
+s = torch.cuda.Stream()                     # does not wait for the default stream
+torch.cuda._sleep(400_000_000)              # a fifth of a second of work on the default stream
+A.paged_step(kv, newd, table, stack, count, kv, count, offsets, positions, slots, status, B, ps, pages, width,
+             max_tokens, stream=s)
+torch.cuda.synchronize()
+st, lens, tab, stk, n, off, pos, sl = O.step([0] * B, new, [[-1] * width for _ in range(B)], list(range(pages)), pages, ps, max_tokens)
+print(json.dumps(dict(status=int(status), want=st, lens=kv.tolist() == lens, table=table.tolist() == tab, count=int(count) == n,
+                      offsets=offsets.tolist() == off, positions=positions.tolist() == pos, slots=slots.tolist() == sl,
+                      error=A.device_error())))
+"""
+
+
+def test_first_growth_on_a_non_blocking_stream():
+    """The counters are zero before the first kernel reads them, whatever the
+    default stream is busy with."""
+    r = in_a_fresh_process(FIRST_CALL)
+    assert r == dict(status=0, want=0, lens=True, table=True, count=True, offsets=True, positions=True, slots=True, error=0)
