@@ -21,7 +21,7 @@ enum DeviceError : int {
     kDevTimeoutFull = 1,   // consumer gave up waiting for a stage to land
     kDevTimeoutEmpty = 2,  // producer gave up waiting for a stage to drain
     kDevTimeoutPeer = 3,   // cross-GPU exchange: the other ranks' states never all arrived
-    kDevBadIndex = 4,      // a position outside its table (read as 0) or a slot outside its pool (skipped)
+    kDevBadIndex = 4,      // a position outside its table (read as 0) or a slot past its pool (not cached)
 };
 
 // Wall-clock budget of one bounded wait (ns).  Real waits last microseconds;

@@ -177,6 +177,27 @@ __device__ __forceinline__ uint32_t code4(const float (&x)[4], const Divisor& d)
     return Code::encode4(y, d.finite);
 }
 
+// K's (which 0) or V's row of token t, with its bias and turned.
+template <int D>
+__device__ __forceinline__ Row8 finish_row(const AppendParams& p, int which, int t, int f0,
+                                           const uint2 (&raw)[2], const uint2 (&bias)[2], bool biased) {
+    Row8 r;
+    unpack4(raw[0], r.lo);
+    unpack4(raw[1], r.hi);
+    if (biased) {
+        Row8 b;
+        unpack4(bias[0], b.lo);
+        unpack4(bias[1], b.hi);
+        add_bias(r, b);
+    }
+    if (!which) {
+        float c[4], s[4];
+        load_turn<D>(p, t, f0, c, s);
+        turn(r, c, s);
+    }
+    return r;
+}
+
 // One run: rows t .. t + n - 1 (n <= 16) of K or V head h go to rows row0 ..
 // of the block at `slot`.  The whole CTA takes part; tops: one word per warp.
 template <int D, class Code>
@@ -216,19 +237,7 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int which, int
         const int j = i * STEP + sub;
         if (j < n) {
             Row8& r = rows[i];
-            unpack4(raw[i][0], r.lo);
-            unpack4(raw[i][1], r.hi);
-            if (biased) {
-                Row8 b;
-                unpack4(bias[0], b.lo);
-                unpack4(bias[1], b.hi);
-                add_bias(r, b);
-            }
-            if (!which) {
-                float cc[4], ss[4];
-                load_turn<D>(p, t + j, f0, cc, ss);
-                turn(r, cc, ss);
-            }
+            r = finish_row<D>(p, which, t + j, f0, raw[i], bias, biased);
             if (y) store_row<D>(y + (t + j) * ys + (size_t)h * D, f0, r);
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = max(top, max(abs_bits(r.lo[e]), abs_bits(r.hi[e])));
@@ -307,16 +316,32 @@ kv8_append_kernel(const __grid_constant__ AppendParams p) {
             bias[1] = *reinterpret_cast<const uint2*>(b + (size_t)h * D + f0 + D / 2);
         }
         // Lane l holds the slot of token t - 15 + l: the tokens that can share
-        // a block with t (lane 31: the last token that can follow t + 15).
+        // a block with t (lane 31: the last token that can follow t + 15); -1 for
+        // a token that is left out, kOutside for a slot past the pool.
+        constexpr long long kOutside = -2;
         auto slots_about = [&](int t) {
             const int tl = t - 15 + lane;
             const long long s = tl >= 0 && tl < p.T ? p.slots[tl] : -1;
             if (s >= pool) record_error(p.err, kDevBadIndex);
-            return s >= 0 && s < pool ? s : -1;
+            return s < 0 ? -1 : s < pool ? s : kOutside;
         };
-        // The window's tokens (lanes 15 ..) that no earlier token shares a block with
         const long long near = slots_about(t0);
         const bool mine = lane >= 15 && lane < 15 + p.window;
+        // Tokens with a slot past the pool are not cached, but their rows are
+        // wanted as the others' are.
+        __half* y = which ? p.v_out : p.k_out;
+        uint32_t outside = y ? __ballot_sync(0xffffffffu, mine && near == kOutside) : 0u;
+#pragma unroll 1
+        for (int c = (threadIdx.x >> 5) * RPW + lane / LPR; outside; --c, outside &= outside - 1) {
+            if (c % (RPW * kAppendWarps) != 0) continue;            // a lane group per token
+            const int t = t0 + __ffs(outside) - 16;
+            const __half* src = (which ? p.v : p.k) + t * p.stride[1 + which] + (size_t)h * D + f0;
+            const uint2 raw[2] = {*reinterpret_cast<const uint2*>(src),
+                                  *reinterpret_cast<const uint2*>(src + D / 2)};
+            store_row<D>(y + t * p.stride[4 + which] + (size_t)h * D, f0,
+                         finish_row<D>(p, which, t, f0, raw, bias, b != nullptr));
+        }
+        // The window's tokens (lanes 15 ..) that no earlier token shares a block with
         const uint32_t mates = __match_any_sync(0xffffffffu, near >= 0 ? near / kKv8Block : -1LL);
         uint32_t firsts = __ballot_sync(0xffffffffu, mine && near >= 0 && __ffs(mates) - 1 == lane);
 #pragma unroll 1

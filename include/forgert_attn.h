@@ -340,9 +340,9 @@ FR_API int fr_paged_step(const int* kv_lens, const int* new_lens, int* block_tab
  * block of zeros) or at least 2^-100.  A call's tokens of one block lie within
  * 16 consecutive tokens, as fr_paged_step lays them out, and are taken in
  * token order.  A block that holds a NaN or an infinity reads back as NaN.
- * A position outside the table (read as 0) or a slot outside the pool (not
- * cached) is recorded: fr_get_device_error then gives device code 4 and
- * FR_ERR_INVALID_ARG.  num_tokens 0 does nothing. */
+ * A position outside the table (read as 0) or a slot past the pool (not
+ * cached; the token's outputs are written) is recorded: fr_get_device_error
+ * then gives device code 4 and FR_ERR_INVALID_ARG.  num_tokens 0 does nothing. */
 FR_API int fr_qkv_rope_append_kv8(const void* q, const void* k, const void* v, void* q_out,
                                   void* k_out, void* v_out, const long long* token_strides,
                                   const void* q_bias, const void* k_bias, const void* v_bias,
