@@ -1420,7 +1420,7 @@ int fr_get_device_error(int clear, int* device_code) {
         int c = 0;
         e = cudaMemcpy(&c, w, sizeof(int), cudaMemcpyDeviceToHost);
         if (e != cudaSuccess) return cuda_fail(e);
-        if (!code) code = c;
+        if (!code || (code == fr::kDevBadIndex && c)) code = c;
         if (clear && c) {
             e = zero_now(w, sizeof(int));
             if (e != cudaSuccess) return cuda_fail(e);

@@ -154,8 +154,11 @@ __device__ __forceinline__ float x_wait_word(const uint64_t* addr, uint64_t w, u
     return __uint_as_float(uint32_t(w));
 }
 
+// The first code stays, but a wait that ran out replaces a bad index: its call
+// did not finish.
 __device__ __forceinline__ void record_error(int* err, int code) {
-    if (err) atomicCAS(err, 0, code);
+    if (err && atomicCAS(err, 0, code) == kDevBadIndex && code != kDevBadIndex)
+        atomicCAS(err, kDevBadIndex, code);
 }
 
 // Named barrier over the consumer warps only (the producer may have exited).

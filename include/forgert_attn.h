@@ -397,8 +397,9 @@ FR_API size_t fr_prefill_workspace_size(int seq_len, int num_heads, int head_dim
 /* Reads (and optionally clears) the current device's in-kernel error words
  * (the regular entry points' and fr_decode_attn_noalloc's): 0 = none,
  * 4 = an index out of range (fr_qkv_rope_append_kv8; FR_ERR_INVALID_ARG is
- * returned), otherwise a bounded wait ran out (FR_ERR_TIMEOUT is returned).  Synchronises the device; creates no state and allocates
- * nothing. */
+ * returned), otherwise a bounded wait ran out (FR_ERR_TIMEOUT is returned,
+ * also when an index was out of range before or after).  Synchronises the
+ * device; creates no state and allocates nothing. */
 FR_API int fr_get_device_error(int clear, int* device_code);
 
 /* Device memory the library has allocated with cudaMalloc on the current
