@@ -52,9 +52,11 @@ struct StepParams {
     int batch, page_size, num_pages, max_blocks, max_tokens;
 };
 
-// Sums that stop at a cap below 2^30: a total past its limit refuses the call
-// whatever it is, and an int never overflows on the way.
-__device__ __forceinline__ int add_capped(int a, int b, int cap) { return min(a + b, cap); }
+// Sums of numbers up to a cap, at most 2^30, that stop there: a total past its
+// limit refuses the call whatever it is.  Two caps make 2^31, past an int.
+__device__ __forceinline__ int add_capped(int a, int b, int cap) {
+    return (int)min((unsigned)a + (unsigned)b, (unsigned)cap);
+}
 
 __device__ __forceinline__ int last_at_most(const int* first, int n, int x) {
     int lo = 0, hi = n - 1;                     // last b with first[b] <= x
