@@ -50,7 +50,8 @@ fr::Kv8View kv8_view(const fr_kv8_cache* c) {
 //     three CTAs (168 registers: the second 8-head tile's state spills at 128)
 //     with three;
 //   DEEP, for calls of few tiles per SM, where warps are few anyway and wait
-//     for memory: fewer CTAs with more steps under way.
+//     for memory: fewer CTAs with more steps under way, and weights of 22 bits
+//     (REST).
 template <int NT, bool DEEP> struct Kv8Shape;
 template <> struct Kv8Shape<1, false> { static constexpr int kCtas = 4, kStages = 2; };
 template <> struct Kv8Shape<2, false> { static constexpr int kCtas = 3, kStages = 3; };
@@ -66,7 +67,8 @@ using Kv8SmemOf = fr::Kv8Smem<D, NT, kv8_mt<D>(), Kv8Shape<NT, DEEP>::kStages, k
 template <int D, int NT, bool DEEP, class Code>
 auto kv8_ptr() {
     using Shape = Kv8Shape<NT, DEEP>;
-    return fr::kv8_decode_kernel<D, NT, kv8_mt<D>(), Shape::kStages, kKv8Warps, Shape::kCtas, Code>;
+    return fr::kv8_decode_kernel<D, NT, kv8_mt<D>(), Shape::kStages, kKv8Warps, Shape::kCtas, DEEP,
+                                 Code>;
 }
 
 template <int D, int NT, bool DEEP, class Code>

@@ -6,10 +6,15 @@
 //   o   = sum_t 2^(s_t log2 e - m) * vscale(block) * vc_t,  l = sum_t 2^(...)
 //   out = o / l  (zeros for an empty sequence)
 // with kc, vc the 8-bit codes.  Scores, m, l and o are fp32.  Codes widen to
-// fp16 exactly; a term 2^s vscale enters the product with V as one fp16
-// (relative rounding 2^-12, below the output's own) on a reference of its own
-// (Kv8State), 2^8 up, so that one as small as 2^-22 of the largest keeps all
-// its bits.  The row sum uses the unrounded probabilities.
+// fp16 exactly; a term 2^s vscale enters the product with V as fp16 on a
+// reference of its own (Kv8State), 2^8 up, so that one as small as 2^-22 of the
+// largest keeps all its bits.  Long calls take that one fp16 (each term rounded
+// by 2^-11 of itself at most, which leaves the outputs 1.2 to 1.3 times as far
+// from the exact ones as their own rounding does); in short calls (REST), where
+// the outputs average fewer terms (1.5 times) and the warps wait for memory, a
+// second product takes the rest of each term: 1 x 512 tokens 8.0 -> 8.1 us, 64
+// of 200 to 300 10.0 -> 10.4, 64 of 1024 to 8192 would be 50.1 -> 52.3.  The row
+// sum uses the unrounded probabilities.
 //
 // Bound: HBM.  2 * D bytes of codes per position and kv head, plus 8 bytes of
 // scales per 16 positions; 4 * D * G operations on them.  Measured, 28 / 4
@@ -221,8 +226,9 @@ struct Kv8Query {
 };
 
 // One step: 16 * MT rows of K at kst and V at vst, of which the first `valid`
-// (>= 1) are positions; sc: their blocks' scales.
-template <int D, int NT, int MT, class Code>
+// (>= 1) are positions; sc: their blocks' scales.  REST: what rounding a weight
+// to fp16 takes off goes into a product of its own.
+template <int D, int NT, int MT, bool REST, class Code>
 __device__ __forceinline__ void consume_kv8(uint32_t kst, uint32_t vst, const float2* sc, int valid,
                                             const Kv8Query<D, NT>& q,
                                             Kv8State<D, NT>& st, float sl2, int lane) {
@@ -341,7 +347,7 @@ __device__ __forceinline__ void consume_kv8(uint32_t kst, uint32_t vst, const fl
 
     // ---- row sums (unrounded), and W^T = P^T vscale as fp16 in the B layout
     // (k = position, n = head)
-    uint32_t wb[MT][NT][2];
+    uint32_t wb[MT][NT][2], wr[MT][NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -351,8 +357,16 @@ __device__ __forceinline__ void consume_kv8(uint32_t kst, uint32_t vst, const fl
                 st.l[nt][c & 1] += fast_exp2(ep[mt][nt][c]);
                 ew[mt][nt][c] = fast_exp2(ew[mt][nt][c]);
             }
-            wb[mt][nt][0] = movmatrix_trans(pack_half2(ew[mt][nt][0], ew[mt][nt][1]));
-            wb[mt][nt][1] = movmatrix_trans(pack_half2(ew[mt][nt][2], ew[mt][nt][3]));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float w0 = ew[mt][nt][2 * e], w1 = ew[mt][nt][2 * e + 1];
+                const uint32_t w = pack_half2(w0, w1);
+                wb[mt][nt][e] = movmatrix_trans(w);
+                if constexpr (REST) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+                    wr[mt][nt][e] = movmatrix_trans(pack_half2(w0 - f.x, w1 - f.y));
+                }
+            }
         }
     }
 
@@ -391,6 +405,11 @@ __device__ __forceinline__ void consume_kv8(uint32_t kst, uint32_t vst, const fl
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
                     mma_16816(st.o[dm][nt], a0, a1, a2, a3, wb[mt][nt][0], wb[mt][nt][1]);
+                if constexpr (REST) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma_16816(st.o[dm][nt], a0, a1, a2, a3, wr[mt][nt][0], wr[mt][nt][1]);
+                }
             }
     }
 }
@@ -613,7 +632,7 @@ __device__ __forceinline__ void kv8_merge(const Kv8DecodeParams& p, float* area,
 // Persistent kernel: grid = C co-resident CTAs of NW warps; see
 // persistent_decode_kernel for units, items, pieces and the merge.
 // ---------------------------------------------------------------------------
-template <int D, int NT, int MT, int STAGES, int NW, int CTAS, class Code>
+template <int D, int NT, int MT, int STAGES, int NW, int CTAS, bool REST, class Code>
 __global__ void __launch_bounds__(32 * NW, CTAS)
 kv8_decode_kernel(const __grid_constant__ Kv8DecodeParams p) {
     constexpr int TILE = 16 * MT * NW;
@@ -724,8 +743,8 @@ kv8_decode_kernel(const __grid_constant__ Kv8DecodeParams p) {
             const uint32_t kst = ring + stage * (2 * S::kStepBytes);
             const int valid = len - ((i0 + tt) * NW + warp) * (16 * MT);
             if (valid > 0)
-                consume_kv8<D, NT, MT, Code>(kst, kst + S::kStepBytes, scales + stage * MT, valid, q, st,
-                                             sl2, lane);
+                consume_kv8<D, NT, MT, REST, Code>(kst, kst + S::kStepBytes, scales + stage * MT, valid, q,
+                                                   st, sl2, lane);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
         }
         cur.advance(seq_start, B, upb, cnt);
