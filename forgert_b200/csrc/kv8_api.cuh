@@ -151,9 +151,10 @@ int kv8_plan(DeviceState* st, int batch, int num_heads, int num_kv_heads, int he
     const long long tiles = (long long)pl.chunk * num_kv_heads * pl.head_groups *
                             std::max(1, (max_kv_len + tile - 1) / tile);
     // The deep shape up to 22 tiles per SM, were every sequence as long as the
-    // longest may be (28 / 4 heads of 128, deep / long shape: one sequence of
-    // 4096 tokens 11.5 / 14.3 us, 64 of up to 300 10.1 / 12.3, 24 of up to 2000
-    // 14.0 / 16.4, 48 of up to 1300 19.4 / 18.2, 64 of up to 8192 57.9 / 49.9).
+    // longest may be (28 / 4 heads of 128, deep / long shape, bursts of calls
+    // and one fp16 weight in both: one sequence of 4096 tokens 11.5 / 14.3 us,
+    // 64 of up to 300 10.1 / 12.3, 24 of up to 2000 14.0 / 16.4, 48 of up to
+    // 1300 19.4 / 18.2, 64 of up to 8192 57.9 / 49.9).
     pl.deep = tiles <= 22LL * st->sm_count;
     const int slot = (head_dim == 64 ? 0 : 8) + (pl.nt - 1) * 4 + (pl.deep ? 2 : 0) + dtype;
     int rc = kv8_dispatch(head_dim, pl.nt, dtype, [&](auto d, auto n, auto code) {

@@ -24,10 +24,10 @@
 // (One warp per run, 64 values a lane: 128 registers and straight-line code
 // that the instruction cache lost, 60 us for 4800 tokens of 28 / 4 heads.)
 //
-// Bound: for prompts issue slots (63 % of the cycles) and the loads' latency at
+// Bound: for prompts issue slots (67 % of the cycles) and the loads' latency at
 // 27 warps per SM - 4800 tokens of 28 / 4 heads of 128, three axes, biases and
 // 16-bit K and V written too, 24 us, 4.0 TB/s; for a decode step latency, four
-// dependent rounds of loads (64 tokens 7 us).
+// dependent rounds of loads (64 tokens 4.5 us in a graph).
 #pragma once
 #include "fr_ptx.cuh"
 #include "decode_kernels.cuh"

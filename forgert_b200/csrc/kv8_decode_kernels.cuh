@@ -16,11 +16,13 @@
 // of 200 to 300 10.0 -> 10.4, 64 of 1024 to 8192 would be 50.1 -> 52.3.  The row
 // sum uses the unrounded probabilities.
 //
-// Bound: HBM.  2 * D bytes of codes per position and kv head, plus 8 bytes of
-// scales per 16 positions; 4 * D * G operations on them.  Measured, 28 / 4
-// heads of 128: 64 sequences of 8192 to 32768 tokens in e4m3 204 us, 6.4 TB/s
-// (0.98 of a copy's rate); of 1024 to 8192 50 us, 5.4 TB/s, of which about 7
-// are launch, first rows, fold and merge; one sequence of 512 tokens 8.
+// Bytes: 2 * D of codes per position and kv head, plus 8 of scales per 16
+// positions; 4 * D * G operations on them.  Measured, 28 / 4 heads of 128: 64
+// sequences of 8192 to 32768 tokens in e4m3 203 us, 6.4 TB/s (0.98 of a copy's
+// rate, bound by HBM), in int8 218; of 1024 to 8192 51 to 56 us, 4.9 to 5.3
+// TB/s, in int8 61 to 66: issue slots (56 and 61 % of the cycles at 16 warps
+// per SM) and latency, about 7 us of them launch, first rows, fold and merge;
+// one sequence of 512 tokens 8 (14 / 2 heads of 64).
 //
 // Decomposition: persistent CTAs take equal shares of the batch's work, as in
 // batched_kernels.cuh (units, items, pieces merged by the contributor that
@@ -202,8 +204,8 @@ struct Kv8State {
 // q of one item as the B operand, in the order that K's words come in: lane
 // (g, t) holds dims (D/4) * t .. of head g, as fp16 pairs.  (int8 codes can
 // also enter integer products, with q in 16-bit fixed point on its head's
-// largest value as two s8 planes: 64 sequences of 8192 to 32768 tokens 210 us
-// instead of 221, but a channel far above the others takes their bits.)
+// largest value as two s8 planes: 64 sequences of 8192 to 32768 tokens 209 us
+// instead of 220, but a channel far above the others takes their bits.)
 template <int D, int NT>
 struct Kv8Query {
     uint32_t b[D / 16][NT][2];

@@ -353,8 +353,9 @@ FR_API int fr_qkv_rope_append_kv8(const void* q, const void* k, const void* v, v
                                   void* stream);
 
 /* Reads slots back as fp16: k_out, v_out [num_slots, num_kv_heads, head_dim]
- * (16-byte aligned; either may be NULL), e.g. a cached prefix for the 16-bit
- * prefill attention.  A slot outside the pool gives zeros. */
+ * (16-byte aligned; either may be NULL), e.g. for an attention of the caller's
+ * own over cached rows (fr_prefill_attn takes queries and keys of one length),
+ * or to look at the cache.  A slot outside the pool gives zeros. */
 FR_API int fr_kv8_gather(const fr_kv8_cache* cache, const long long* slots, void* k_out,
                          void* v_out, int num_slots, void* stream);
 
@@ -370,7 +371,12 @@ FR_API int fr_kv8_gather(const fr_kv8_cache* cache, const long long* slots, void
  *                max_kv_len is cut to it
  *   max_kv_len   host upper bound of kv_lens, <= max_blocks_per_seq * page_size
  * Rows past a sequence's end are never used, whatever they hold.  A NaN or
- * infinite scale of a used block makes the outputs it enters NaN.  The result
+ * infinite scale of a used block makes the outputs it enters NaN.  Scores and
+ * sums are fp32.  A short call is off by the rounding of its outputs; a long
+ * one also rounds each weight to fp16 (2^-11 of itself).  A call is long when
+ * batch * num_kv_heads sequences of max_kv_len, in tiles of 8192 / head_dim
+ * positions (once more for each 16 query heads of a group above 16), make more
+ * than 22 tiles per SM, at most 512 sequences counted.  The result
  * does not depend on which CTA merges: equal inputs give equal bits. */
 FR_API int fr_decode_attn_paged_kv8(const void* q, long long q_stride, const fr_kv8_cache* cache,
                                     const int* block_table, const int* kv_lens, void* out,
