@@ -79,7 +79,11 @@ class Server:
                      self.kv_lens, self.free_count, self.offsets, self.positions, self.slots,
                      self.status, self.rows, self.page_size, self.num_pages, self.width,
                      max_tokens, stream=stream)
-        with torch.cuda.stream(torch.cuda.default_stream() if stream is None else stream):
+        if not stream:
+            stream = torch.cuda.default_stream()
+        elif isinstance(stream, int):
+            stream = torch.cuda.ExternalStream(stream)
+        with torch.cuda.stream(stream):
             first = self.offsets[:-1]
             at = torch.where(self.offsets[1:] > first, first, self.max_tokens)
             torch.index_select(self.positions, 0, at, out=self.row_positions)
