@@ -61,166 +61,23 @@ constexpr int kKv8Warps = 4;
 template <int D> constexpr int kv8_mt() { return 128 / D; }
 constexpr int kv8_tile(int head_dim) { return 16 * (128 / head_dim) * kKv8Warps; }
 
-template <int D, int NT, bool DEEP>
-using Kv8SmemOf = fr::Kv8Smem<D, NT, kv8_mt<D>(), Kv8Shape<NT, DEEP>::kStages, kKv8Warps>;
-
 template <int D, int NT, bool DEEP, class Code>
-auto kv8_ptr() {
-    using Shape = Kv8Shape<NT, DEEP>;
-    return fr::kv8_decode_kernel<D, NT, kv8_mt<D>(), Shape::kStages, kKv8Warps, Shape::kCtas, DEEP,
-                                 Code>;
-}
+using Kv8FormatOf = fr::Kv8Format<D, NT, kv8_mt<D>(), Kv8Shape<NT, DEEP>::kStages, kKv8Warps,
+                                  Kv8Shape<NT, DEEP>::kCtas, DEEP, Code>;
 
-template <int D, int NT, bool DEEP, class Code>
-int prepare_kv8(DeviceState* st, int slot) {
+// Sets a decode kernel's shared memory and asks for its CTAs per SM, once.
+template <class F>
+int prepare_cached(int* occ) {
     std::lock_guard<std::mutex> lk(g_prep_mu);
-    if (st->kv8_occ[slot]) return FR_OK;
-    const int bytes = static_cast<int>(Kv8SmemOf<D, NT, DEEP>::kBytes);
-    auto fn = kv8_ptr<D, NT, DEEP, Code>();
+    if (*occ) return FR_OK;
+    const int bytes = static_cast<int>(F::Smem::kBytes);
+    auto fn = fr::cached_decode_kernel<F>;
     cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return cuda_fail(e);
     int n = 0;
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, 32 * kKv8Warps, bytes);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, 32 * F::kNW, bytes);
     if (e != cudaSuccess) return cuda_fail(e);
-    st->kv8_occ[slot] = std::max(1, n);
-    return FR_OK;
-}
-
-template <int D, int NT, bool DEEP, class Code>
-int launch_kv8(const fr::Kv8DecodeParams& kp, int ctas, cudaStream_t s) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, 1, 1);
-    cfg.blockDim = dim3(32 * kKv8Warps, 1, 1);
-    cfg.dynamicSmemBytes = Kv8SmemOf<D, NT, DEEP>::kBytes;
-    cfg.stream = s;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_ptr<D, NT, DEEP, Code>(), kp);
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    if (e == cudaSuccess) e = cudaGetLastError();
-    return e == cudaSuccess ? FR_OK : cuda_fail(e);
-}
-
-// f(D, NT, Code) for the sizes and type at hand.
-template <class F>
-int kv8_dispatch(int head_dim, int nt, int dtype, F f) {
-    using std::integral_constant;
-    auto with_code = [&](auto d, auto n) {
-        return dtype == FR_KV8_INT8 ? f(d, n, fr::Int8Code()) : f(d, n, fr::E4m3Code());
-    };
-    auto with_nt = [&](auto d) {
-        return nt == 1 ? with_code(d, integral_constant<int, 1>())
-                       : with_code(d, integral_constant<int, 2>());
-    };
-    return head_dim == 64 ? with_nt(integral_constant<int, 64>())
-                          : with_nt(integral_constant<int, 128>());
-}
-
-// Counters of a call: one per unit, then one per partial slot.
-constexpr int kKv8Units = kMaxUnits / 2;
-
-// Sequences per launch: their lengths' prefix fits shared memory, their units
-// the counters, their tiles the kernel's 32-bit tile numbers.  0 = not even one.
-int kv8_chunk(int batch, int num_kv_heads, int head_groups, int head_dim, int max_kv_len) {
-    const long long upb = (long long)num_kv_heads * head_groups;
-    const int tile = kv8_tile(head_dim);
-    const long long tiles = std::max(1, (max_kv_len + tile - 1) / tile);
-    const long long n = std::min({(long long)fr::kPersistMaxBatch, kKv8Units / upb,
-                                  ((1LL << 29) - 1) / (upb * tiles), (long long)batch});
-    return (int)n;
-}
-
-struct Kv8Plan {
-    int nt = 1, head_groups = 1, chunk = 0, ctas = 0;
-    bool deep = false;
-    size_t ws_bytes = 0;
-};
-
-int kv8_plan(DeviceState* st, int batch, int num_heads, int num_kv_heads, int head_dim,
-             int max_kv_len, int dtype, Kv8Plan* out) {
-    Kv8Plan pl;
-    const int group = num_heads / num_kv_heads;
-    pl.nt = group <= 8 ? 1 : 2;
-    pl.head_groups = (group + 8 * pl.nt - 1) / (8 * pl.nt);
-    pl.chunk = kv8_chunk(batch, num_kv_heads, pl.head_groups, head_dim, max_kv_len);
-    if (pl.chunk <= 0) return FR_ERR_INVALID_ARG;
-    const int tile = kv8_tile(head_dim);
-    const long long tiles = (long long)pl.chunk * num_kv_heads * pl.head_groups *
-                            std::max(1, (max_kv_len + tile - 1) / tile);
-    // The deep shape up to 22 tiles per SM, were every sequence as long as the
-    // longest may be (28 / 4 heads of 128, deep / long shape, bursts of calls
-    // and one fp16 weight in both: one sequence of 4096 tokens 11.5 / 14.3 us,
-    // 64 of up to 300 10.1 / 12.3, 24 of up to 2000 14.0 / 16.4, 48 of up to
-    // 1300 19.4 / 18.2, 64 of up to 8192 57.9 / 49.9).
-    pl.deep = tiles <= 22LL * st->sm_count;
-    const int slot = (head_dim == 64 ? 0 : 8) + (pl.nt - 1) * 4 + (pl.deep ? 2 : 0) + dtype;
-    int rc = kv8_dispatch(head_dim, pl.nt, dtype, [&](auto d, auto n, auto code) {
-        constexpr int D = decltype(d)::value, NT = decltype(n)::value;
-        return pl.deep ? prepare_kv8<D, NT, true, decltype(code)>(st, slot)
-                       : prepare_kv8<D, NT, false, decltype(code)>(st, slot);
-    });
-    if (rc != FR_OK) return rc;
-    pl.ctas = (int)std::max<long long>(
-        1, std::min<long long>((long long)st->sm_count * st->kv8_occ[slot], tiles));
-    pl.ws_bytes = kCounterBytes + (size_t)2 * pl.ctas * 8 * pl.nt * (head_dim + 2) * sizeof(float);
-    *out = pl;
-    return FR_OK;
-}
-
-int run_kv8(const void* q, long long q_stride, const fr_kv8_cache* cache, const int* block_table,
-            const int* kv_lens, void* out, int batch, int num_heads, int max_blocks,
-            int max_kv_len, cudaStream_t s) {
-    DeviceState* st = nullptr;
-    int rc = get_state(&st);
-    if (rc != FR_OK) return rc;
-    const int Hkv = cache->num_kv_heads, D = cache->head_dim;
-    const int len = std::max(1, max_kv_len);
-    Kv8Plan pl;
-    rc = kv8_plan(st, batch, num_heads, Hkv, D, len, cache->dtype, &pl);
-    if (rc != FR_OK) return rc;
-    rc = ensure_workspace(st, pl.ws_bytes, s);
-    if (rc != FR_OK) return rc;
-    fr::Kv8DecodeParams p;
-    std::memset(&p, 0, sizeof(p));
-    p.cache = kv8_view(cache);
-    p.q_stride = q_stride;
-    p.H = num_heads;
-    p.G = num_heads / Hkv;
-    p.head_groups = pl.head_groups;
-    p.bt_stride = max_blocks;
-    p.max_len = max_kv_len;
-    p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)D));
-    p.counters = static_cast<int*>(st->ws);
-    p.max_units = kKv8Units;
-    p.part_ml = reinterpret_cast<float*>(static_cast<char*>(st->ws) + kCounterBytes);
-    p.part_acc = p.part_ml + (size_t)2 * pl.ctas * 8 * pl.nt * 2;
-    // At least two tiles per CTA before SMs get more than one.  A unit's start
-    // and its merge are charged as one tile each (four each, which suits the
-    // 16-bit kernel's longer tiles, left too few CTAs to short calls: one
-    // sequence of 2048 tokens 18.6 us instead of 10.6), and units of up to six
-    // tiles are not cut: 64 sequences of 200 to 300 tokens 17.4 -> 12.4 us, no
-    // call measured slower.
-    p.min_tiles_per_cta = 2;
-    p.min_ctas = st->sm_count;
-    p.item_cost = 1;
-    p.merge_cost = 1;
-    p.whole_tiles = 6;
-    for (int b = 0; b < batch; b += pl.chunk) {
-        p.batch = std::min(pl.chunk, batch - b);
-        p.q = static_cast<const __half*>(q) + (size_t)b * q_stride;
-        p.out = static_cast<__half*>(out) + (size_t)b * num_heads * D;
-        p.kv_lens = kv_lens + b;
-        p.block_table = block_table + (size_t)b * max_blocks;
-        rc = kv8_dispatch(D, pl.nt, cache->dtype, [&](auto d, auto n, auto code) {
-            constexpr int kD = decltype(d)::value, NT = decltype(n)::value;
-            return pl.deep ? launch_kv8<kD, NT, true, decltype(code)>(p, pl.ctas, s)
-                           : launch_kv8<kD, NT, false, decltype(code)>(p, pl.ctas, s);
-        });
-        if (rc != FR_OK) return rc;
-    }
+    *occ = std::max(1, n);
     return FR_OK;
 }
 
@@ -244,6 +101,131 @@ int launch_plain(void (*fn)(Args...), unsigned grid, unsigned block, size_t smem
     g_launches.fetch_add(1, std::memory_order_relaxed);
     if (e == cudaSuccess) e = cudaGetLastError();
     return e == cudaSuccess ? FR_OK : cuda_fail(e);
+}
+
+template <class F>
+int launch_cached(const typename F::Params& p, int ctas, cudaStream_t s) {
+    return launch_plain(fr::cached_decode_kernel<F>, (unsigned)ctas, 32 * F::kNW, F::Smem::kBytes, s, p);
+}
+
+// f(D, NT, Code) for the sizes and type at hand.
+template <class F>
+int kv8_dispatch(int head_dim, int nt, int dtype, F f) {
+    using std::integral_constant;
+    auto with_code = [&](auto d, auto n) {
+        return dtype == FR_KV8_INT8 ? f(d, n, fr::Int8Code()) : f(d, n, fr::E4m3Code());
+    };
+    auto with_nt = [&](auto d) {
+        return nt == 1 ? with_code(d, integral_constant<int, 1>())
+                       : with_code(d, integral_constant<int, 2>());
+    };
+    return head_dim == 64 ? with_nt(integral_constant<int, 64>())
+                          : with_nt(integral_constant<int, 128>());
+}
+
+// Counters of a call: one per unit, then one per partial slot.
+constexpr int kCachedUnits = kMaxUnits / 2;
+
+// Sequences per launch: their lengths' prefix fits shared memory, their units
+// the counters, their tiles the kernel's 32-bit tile numbers.  0 = not even one.
+int cached_chunk(int batch, int num_kv_heads, int head_groups, int tile, int max_kv_len) {
+    const long long upb = (long long)num_kv_heads * head_groups;
+    const long long tiles = std::max(1, (max_kv_len + tile - 1) / tile);
+    const long long n = std::min({(long long)fr::kPersistMaxBatch, kCachedUnits / upb,
+                                  ((1LL << 29) - 1) / (upb * tiles), (long long)batch});
+    return (int)n;
+}
+
+struct CachedPlan {
+    int nt = 1, head_groups = 1, chunk = 0, ctas = 0;
+    bool deep = false;
+    size_t ws_bytes = 0;
+};
+
+int kv8_plan(DeviceState* st, int batch, int num_heads, int num_kv_heads, int head_dim,
+             int max_kv_len, int dtype, CachedPlan* out) {
+    CachedPlan pl;
+    const int group = num_heads / num_kv_heads;
+    pl.nt = group <= 8 ? 1 : 2;
+    pl.head_groups = (group + 8 * pl.nt - 1) / (8 * pl.nt);
+    const int tile = kv8_tile(head_dim);
+    pl.chunk = cached_chunk(batch, num_kv_heads, pl.head_groups, tile, max_kv_len);
+    if (pl.chunk <= 0) return FR_ERR_INVALID_ARG;
+    const long long tiles = (long long)pl.chunk * num_kv_heads * pl.head_groups *
+                            std::max(1, (max_kv_len + tile - 1) / tile);
+    // The deep shape up to 22 tiles per SM, were every sequence as long as the
+    // longest may be (28 / 4 heads of 128, deep / long shape, bursts of calls
+    // and one fp16 weight in both: one sequence of 4096 tokens 11.5 / 14.3 us,
+    // 64 of up to 300 10.1 / 12.3, 24 of up to 2000 14.0 / 16.4, 48 of up to
+    // 1300 19.4 / 18.2, 64 of up to 8192 57.9 / 49.9).
+    pl.deep = tiles <= 22LL * st->sm_count;
+    const int slot = (head_dim == 64 ? 0 : 8) + (pl.nt - 1) * 4 + (pl.deep ? 2 : 0) + dtype;
+    int rc = kv8_dispatch(head_dim, pl.nt, dtype, [&](auto d, auto n, auto code) {
+        constexpr int D = decltype(d)::value, NT = decltype(n)::value;
+        int* occ = &st->kv8_occ[slot];
+        return pl.deep ? prepare_cached<Kv8FormatOf<D, NT, true, decltype(code)>>(occ)
+                       : prepare_cached<Kv8FormatOf<D, NT, false, decltype(code)>>(occ);
+    });
+    if (rc != FR_OK) return rc;
+    pl.ctas = (int)std::max<long long>(
+        1, std::min<long long>((long long)st->sm_count * st->kv8_occ[slot], tiles));
+    pl.ws_bytes = kCounterBytes + (size_t)2 * pl.ctas * 8 * pl.nt * (head_dim + 2) * sizeof(float);
+    *out = pl;
+    return FR_OK;
+}
+
+int run_kv8(const void* q, long long q_stride, const fr_kv8_cache* cache, const int* block_table,
+            const int* kv_lens, void* out, int batch, int num_heads, int max_blocks,
+            int max_kv_len, cudaStream_t s) {
+    DeviceState* st = nullptr;
+    int rc = get_state(&st);
+    if (rc != FR_OK) return rc;
+    const int Hkv = cache->num_kv_heads, D = cache->head_dim;
+    const int len = std::max(1, max_kv_len);
+    CachedPlan pl;
+    rc = kv8_plan(st, batch, num_heads, Hkv, D, len, cache->dtype, &pl);
+    if (rc != FR_OK) return rc;
+    rc = ensure_workspace(st, pl.ws_bytes, s);
+    if (rc != FR_OK) return rc;
+    fr::CachedDecodeParams<fr::Kv8View> p;
+    std::memset(&p, 0, sizeof(p));
+    p.cache = kv8_view(cache);
+    p.q_stride = q_stride;
+    p.H = num_heads;
+    p.G = num_heads / Hkv;
+    p.head_groups = pl.head_groups;
+    p.bt_stride = max_blocks;
+    p.max_len = max_kv_len;
+    p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)D));
+    p.counters = static_cast<int*>(st->ws);
+    p.max_units = kCachedUnits;
+    p.part_ml = reinterpret_cast<float*>(static_cast<char*>(st->ws) + kCounterBytes);
+    p.part_acc = p.part_ml + (size_t)2 * pl.ctas * 8 * pl.nt * 2;
+    // At least two tiles per CTA before SMs get more than one.  A unit's start
+    // and its merge are charged as one tile each (four each, which suits the
+    // 16-bit kernel's longer tiles, left too few CTAs to short calls: one
+    // sequence of 2048 tokens 18.6 us instead of 10.6), and units of up to six
+    // tiles are not cut: 64 sequences of 200 to 300 tokens 17.4 -> 12.4 us, no
+    // call measured slower.
+    p.min_tiles_per_cta = 2;
+    p.min_ctas = st->sm_count;
+    p.item_cost = 1;
+    p.merge_cost = 1;
+    p.whole_tiles = 6;
+    for (int b = 0; b < batch; b += pl.chunk) {
+        p.batch = std::min(pl.chunk, batch - b);
+        p.q = static_cast<const __half*>(q) + (size_t)b * q_stride;
+        p.out = static_cast<__half*>(out) + (size_t)b * num_heads * D;
+        p.kv_lens = kv_lens + b;
+        p.block_table = block_table + (size_t)b * max_blocks;
+        rc = kv8_dispatch(D, pl.nt, cache->dtype, [&](auto d, auto n, auto code) {
+            constexpr int kD = decltype(d)::value, NT = decltype(n)::value;
+            return pl.deep ? launch_cached<Kv8FormatOf<kD, NT, true, decltype(code)>>(p, pl.ctas, s)
+                           : launch_cached<Kv8FormatOf<kD, NT, false, decltype(code)>>(p, pl.ctas, s);
+        });
+        if (rc != FR_OK) return rc;
+    }
+    return FR_OK;
 }
 
 }  // namespace
@@ -455,7 +437,7 @@ size_t fr_kv8_workspace_size(int batch, int num_heads, int num_kv_heads, int hea
         DeviceState* st = nullptr;
         int rc = get_state(&st);
         for (int dtype : {FR_KV8_INT8, FR_KV8_E4M3}) {
-            Kv8Plan pl;
+            CachedPlan pl;
             if (rc == FR_OK)
                 rc = kv8_plan(st, batch, num_heads, num_kv_heads, head_dim,
                               std::max(1, max_kv_len), dtype, &pl);
