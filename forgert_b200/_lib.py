@@ -23,6 +23,7 @@ FR_ERR_SCRATCH_LIMIT = 7
 FR_KV8_INT8 = 0
 FR_KV8_E4M3 = 1
 FR_KV8_BLOCK = 16
+FR_KV4_GROUP = 64
 
 FR_STEP_OK = 0
 FR_STEP_NO_PAGES = 1
@@ -45,7 +46,18 @@ class Kv8CacheStruct(ctypes.Structure):
                 ("row_stride", ctypes.c_longlong)]
 
 
+class Kv4CacheStruct(ctypes.Structure):
+    """fr_kv4_cache of include/forgert_attn.h."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("scales", _vp), ("num_pages", _i), ("page_size", _i),
+                ("num_kv_heads", _i), ("head_dim", _i), ("page_stride", ctypes.c_longlong),
+                ("head_stride", ctypes.c_longlong), ("row_stride", ctypes.c_longlong)]
+
+
 _kv8 = ctypes.POINTER(Kv8CacheStruct)
+_kv4 = ctypes.POINTER(Kv4CacheStruct)
+_append = [_vp, _vp, _vp, _vp, _vp, _vp, ctypes.POINTER(ctypes.c_longlong), _vp, _vp, _vp, _vp, _vp,
+           _i, _vp, _i, ctypes.c_char_p, _vp]
 SIGNATURES = {
     "fr_decode_attn": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "fr_decode_attn_noalloc": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
@@ -90,6 +102,12 @@ SIGNATURES = {
     "fr_decode_attn_paged_kv8": (_i, [_vp, ctypes.c_longlong, _kv8, _vp, _vp, _vp, _i, _i, _i, _i,
                                       _vp]),
     "fr_kv8_workspace_size": (ctypes.c_size_t, [_i, _i, _i, _i, _i]),
+    "fr_qkv_rope_append_paged": (_i, _append + [_vp, _vp] + [_i] * 6 + [_vp]),
+    "fr_qkv_rope_append_kv4": (_i, _append + [_kv4, _i, _i, _vp]),
+    "fr_kv4_gather": (_i, [_kv4, _vp, _vp, _vp, _i, _vp]),
+    "fr_decode_attn_paged_kv4": (_i, [_vp, ctypes.c_longlong, _kv4, _vp, _vp, _vp, _i, _i, _i, _i,
+                                      _vp]),
+    "fr_kv4_workspace_size": (ctypes.c_size_t, [_i, _i, _i, _i, _i]),
     "fr_copy_async": (_i, [_vp, _vp, ctypes.c_size_t, _vp]),
 }
 

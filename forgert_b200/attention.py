@@ -23,7 +23,8 @@ __all__ = [
     "rope_tables_device",
     "rope_append", "reserve_workspace", "decode_workspace_size", "device_error",
     "KV8Cache", "paged_step", "qkv_rope_append_kv8", "kv8_gather", "decode_attn_paged_kv8",
-    "kv8_workspace_size",
+    "kv8_workspace_size", "qkv_rope_append_paged", "KV4Cache", "qkv_rope_append_kv4", "kv4_gather",
+    "decode_attn_paged_kv4", "kv4_workspace_size",
 ]
 
 
@@ -299,6 +300,128 @@ def decode_attn_paged_kv8(q, cache: KV8Cache, block_table, kv_lens, out, batch: 
 def kv8_workspace_size(batch: int, num_heads: int, num_kv_heads: int, head_dim: int,
                        max_kv_len: int) -> int:
     return int(load().fr_kv8_workspace_size(batch, num_heads, num_kv_heads, head_dim,
+                                            max_kv_len))
+
+
+def _append_extras(head_dim: int, freq_axis, token_strides):
+    if freq_axis is not None and len(freq_axis) != head_dim // 2:
+        raise ValueError("freq_axis must name an axis for each of the head_dim / 2 frequencies")
+    return None if token_strides is None else (ctypes.c_longlong * 6)(*token_strides)
+
+
+def qkv_rope_append_paged(q, k, v, q_out, k_out, v_out, cos_tab, sin_tab, positions, slots,
+                          k_pages, v_pages, page_size: int, num_pages: int, num_tokens: int,
+                          num_heads: int, num_kv_heads: int, head_dim: int, table_rows: int,
+                          q_bias=None, k_bias=None, v_bias=None, num_axes: int = 1,
+                          freq_axis: bytes | None = None, token_strides=None,
+                          stream=None) -> None:
+    """Bias + RoPE on q/k and K/V rows written at `slots` of the 16-bit pages
+    [num_pages, page_size, num_kv_heads, head_dim] that decode_attn_paged reads
+    (one launch).  positions int32 [num_axes, num_tokens], freq_axis the axis of
+    each of the head_dim / 2 frequencies; k_out / v_out may be None and every
+    output its input; token_strides: halves between tokens of q, k, v, q_out,
+    k_out, v_out (multiples of 8)."""
+    lib = load()
+    rc = lib.fr_qkv_rope_append_paged(
+        _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(v_out),
+        _append_extras(head_dim, freq_axis, token_strides), _ptr(q_bias), _ptr(k_bias),
+        _ptr(v_bias), _ptr(cos_tab), _ptr(sin_tab), table_rows, _ptr(positions), num_axes,
+        freq_axis, _ptr(slots), _ptr(k_pages), _ptr(v_pages), page_size, num_pages, num_tokens,
+        num_heads, num_kv_heads, head_dim, _stream(stream))
+    if rc:
+        check("fr_qkv_rope_append_paged", rc)
+
+
+class KV4Cache:
+    """A paged cache held in 4 bits (fr_kv4_cache): a value is code * scale + bias.
+
+    k, v [num_pages, num_kv_heads, page_size, head_dim / 2] torch.uint8, two
+    codes to a byte, contiguous in the last dimension and both of the same
+    strides, else of any; scales [num_pages, num_kv_heads, page_size, 2,
+    head_dim / 64, 2] fp16, contiguous (for each row of K and of V the scale and
+    bias of each 64 dims).  The cache is the caller's memory: this keeps the
+    tensors and their layout.
+    """
+
+    def __init__(self, k, v, scales):
+        import torch
+
+        if k.dtype != torch.uint8 or v.dtype != torch.uint8:
+            raise ValueError("k and v must be torch.uint8")
+        if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or k.stride(3) != 1:
+            raise ValueError("k and v must be [num_pages, num_kv_heads, page_size, head_dim / 2] "
+                             "with equal strides, contiguous in the last dimension")
+        pages, heads, rows, width = k.shape
+        dim = 2 * width
+        if (scales.dtype != torch.float16 or not scales.is_contiguous() or
+                tuple(scales.shape) != (pages, heads, rows, 2, dim // _lib.FR_KV4_GROUP, 2)):
+            raise ValueError("scales must be contiguous fp16 "
+                             "[num_pages, num_kv_heads, page_size, 2, head_dim / 64, 2]")
+        self.k, self.v, self.scales = k, v, scales
+        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = pages, heads, rows, dim
+        # a dimension of one element never steps: give it a stride the checks accept
+        strides = [k.stride(i) if k.shape[i] > 1 else -(-width // 16) * 16 for i in range(3)]
+        self._struct = _lib.Kv4CacheStruct(
+            _ptr(k), _ptr(v), _ptr(scales), pages, rows, heads, dim, *strides)
+        self._ref = ctypes.byref(self._struct)
+
+    @classmethod
+    def empty(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
+              device="cuda"):
+        """A cache in fresh memory, page and head outermost."""
+        import torch
+
+        k = torch.empty((num_pages, num_kv_heads, page_size, head_dim // 2), dtype=torch.uint8,
+                        device=device)
+        scales = torch.empty((num_pages, num_kv_heads, page_size, 2,
+                              head_dim // _lib.FR_KV4_GROUP, 2), dtype=torch.float16, device=device)
+        return cls(k, torch.empty_like(k), scales)
+
+
+def qkv_rope_append_kv4(q, k, v, q_out, k_out, v_out, cos_tab, sin_tab, positions, slots,
+                        cache: KV4Cache, num_tokens: int, num_heads: int, table_rows: int,
+                        q_bias=None, k_bias=None, v_bias=None, num_axes: int = 1,
+                        freq_axis: bytes | None = None, token_strides=None, stream=None) -> None:
+    """Bias + RoPE on q/k and K/V coded into the 4-bit cache at `slots` (one
+    launch); the other arguments as in qkv_rope_append_paged."""
+    lib = load()
+    rc = lib.fr_qkv_rope_append_kv4(
+        _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_out), _ptr(v_out),
+        _append_extras(cache.head_dim, freq_axis, token_strides), _ptr(q_bias), _ptr(k_bias),
+        _ptr(v_bias), _ptr(cos_tab), _ptr(sin_tab), table_rows, _ptr(positions), num_axes,
+        freq_axis, _ptr(slots), cache._ref, num_tokens, num_heads, _stream(stream))
+    if rc:
+        check("fr_qkv_rope_append_kv4", rc)
+
+
+def kv4_gather(cache: KV4Cache, slots, k_out, v_out, num_slots: int, stream=None) -> None:
+    """Reads slots back as fp16 [num_slots, num_kv_heads, head_dim] (either
+    output may be None); a slot outside the pool gives zeros."""
+    lib = load()
+    rc = lib.fr_kv4_gather(cache._ref, _ptr(slots), _ptr(k_out), _ptr(v_out), num_slots,
+                           _stream(stream))
+    if rc:
+        check("fr_kv4_gather", rc)
+
+
+def decode_attn_paged_kv4(q, cache: KV4Cache, block_table, kv_lens, out, batch: int,
+                          num_heads: int, max_blocks_per_seq: int, max_kv_len: int,
+                          q_stride: int = 0, stream=None) -> None:
+    """Decode attention, one token per sequence, over the 4-bit paged cache:
+    q/out [batch, num_heads, head_dim] fp16 (q_stride halves between the
+    sequences' q, 0 = contiguous), block_table int32 [batch,
+    max_blocks_per_seq], kv_lens int32 [batch]."""
+    lib = load()
+    rc = lib.fr_decode_attn_paged_kv4(
+        _ptr(q), q_stride, cache._ref, _ptr(block_table), _ptr(kv_lens), _ptr(out), batch,
+        num_heads, max_blocks_per_seq, max_kv_len, _stream(stream))
+    if rc:
+        check("fr_decode_attn_paged_kv4", rc)
+
+
+def kv4_workspace_size(batch: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                       max_kv_len: int) -> int:
+    return int(load().fr_kv4_workspace_size(batch, num_heads, num_kv_heads, head_dim,
                                             max_kv_len))
 
 

@@ -12,6 +12,8 @@
 #include "copy_kernels.cuh"
 #include "kv8_decode_kernels.cuh"
 #include "kv8_append_kernels.cuh"
+#include "kv4_decode_kernels.cuh"
+#include "paged_append_kernels.cuh"
 #include "paged_step_kernels.cuh"
 #include "../../include/forgert_attn.h"
 
@@ -64,6 +66,7 @@ struct DeviceState {
     int resident[4][5] = {{-1, -1, -1, -1, -1}, {-1, -1, -1, -1, -1}, {-1, -1, -1, -1, -1},
                           {-1, -1, -1, -1, -1}};   // co-resident clusters per (slot, log2 size)
     int kv8_occ[16] = {0};       // CTAs/SM of the 8-bit decode kernels (0 = not prepared)
+    int kv4_occ[8] = {0};        // ... and of the 4-bit ones
     bool step_ready = false;     // paged_step_kernel's shared-memory attribute set
     int resident_g[4][2] = {{-1, -1}, {-1, -1}, {-1, -1}, {-1, -1}};   // grouped form, 8 / 16
 };
@@ -1681,3 +1684,4 @@ extern "C" int fr_decode_attn_noalloc(const void* q, const void* k_cache, const 
 }
 
 #include "kv8_api.cuh"
+#include "kv4_api.cuh"

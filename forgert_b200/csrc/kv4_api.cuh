@@ -1,0 +1,325 @@
+// kv4_api.cuh - entry points of the 4-bit paged cache and of the 16-bit pages'
+// append (included by capi.cu after kv8_api.cuh, whose launch and planning
+// helpers they share).
+#pragma once
+
+namespace {
+
+constexpr int kPageRows = 16;           // pages hold whole blocks of this many rows
+
+int check_kv4(const fr_kv4_cache* c) {
+    if (!c || !c->k || !c->v || !c->scales || c->num_pages <= 0 || c->page_size <= 0 ||
+        c->page_size % kPageRows != 0 || c->num_kv_heads <= 0)
+        return FR_ERR_INVALID_ARG;
+    if (c->head_dim != 64 && c->head_dim != 128) return FR_ERR_UNSUPPORTED;
+    const long long limit = 1LL << 40;
+    for (long long s : {c->page_stride, c->head_stride, c->row_stride})
+        if (s < c->head_dim / 2 || s >= limit) return FR_ERR_INVALID_ARG;
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->scales, 16) ||
+        ((c->page_stride | c->head_stride | c->row_stride) & 15))
+        return FR_ERR_MISALIGNED;
+    return FR_OK;
+}
+
+fr::Kv4View kv4_view(const fr_kv4_cache* c) {
+    fr::Kv4View v;
+    v.k = static_cast<uint8_t*>(c->k);
+    v.v = static_cast<uint8_t*>(c->v);
+    v.scales = static_cast<__half*>(c->scales);
+    v.num_pages = c->num_pages;
+    v.page_size = c->page_size;
+    v.Hkv = c->num_kv_heads;
+    v.page_stride = c->page_stride;
+    v.head_stride = c->head_stride;
+    v.row_stride = c->row_stride;
+    return v;
+}
+
+// Shapes of the decode kernel: four warps, steps of 32 rows.
+template <int D, int NT, bool DEEP> struct Kv4Shape;
+template <> struct Kv4Shape<128, 1, false> { static constexpr int kMT = 2, kCtas = 3, kStages = 3; };
+template <> struct Kv4Shape<128, 1, true> { static constexpr int kMT = 2, kCtas = 2, kStages = 4; };
+template <> struct Kv4Shape<128, 2, false> { static constexpr int kMT = 2, kCtas = 2, kStages = 4; };
+template <> struct Kv4Shape<128, 2, true> { static constexpr int kMT = 2, kCtas = 2, kStages = 4; };
+template <> struct Kv4Shape<64, 1, false> { static constexpr int kMT = 2, kCtas = 4, kStages = 4; };
+template <> struct Kv4Shape<64, 1, true> { static constexpr int kMT = 2, kCtas = 3, kStages = 4; };
+template <> struct Kv4Shape<64, 2, false> { static constexpr int kMT = 2, kCtas = 2, kStages = 4; };
+template <> struct Kv4Shape<64, 2, true> { static constexpr int kMT = 2, kCtas = 2, kStages = 4; };
+constexpr int kKv4Warps = 4;
+constexpr int kKv4Tile = 16 * 2 * kKv4Warps;
+
+template <int D, int NT, bool DEEP>
+using Kv4FormatOf = fr::Kv4Format<D, NT, Kv4Shape<D, NT, DEEP>::kMT, Kv4Shape<D, NT, DEEP>::kStages,
+                                  kKv4Warps, Kv4Shape<D, NT, DEEP>::kCtas, DEEP>;
+
+// f(Format) for the sizes at hand.
+template <class F>
+int kv4_dispatch(int head_dim, int nt, bool deep, F f) {
+    auto with_nt = [&](auto d, auto n) {
+        constexpr int D = decltype(d)::value, NT = decltype(n)::value;
+        return deep ? f(Kv4FormatOf<D, NT, true>()) : f(Kv4FormatOf<D, NT, false>());
+    };
+    auto with_d = [&](auto d) {
+        return nt == 1 ? with_nt(d, std::integral_constant<int, 1>())
+                       : with_nt(d, std::integral_constant<int, 2>());
+    };
+    return head_dim == 64 ? with_d(std::integral_constant<int, 64>())
+                          : with_d(std::integral_constant<int, 128>());
+}
+
+int kv4_plan(DeviceState* st, int batch, int num_heads, int num_kv_heads, int head_dim,
+             int max_kv_len, CachedPlan* out) {
+    CachedPlan pl;
+    const int group = num_heads / num_kv_heads;
+    pl.nt = group <= 8 ? 1 : 2;
+    pl.head_groups = (group + 8 * pl.nt - 1) / (8 * pl.nt);
+    pl.chunk = cached_chunk(batch, num_kv_heads, pl.head_groups, kKv4Tile, max_kv_len);
+    if (pl.chunk <= 0) return FR_ERR_INVALID_ARG;
+    const long long tiles = (long long)pl.chunk * num_kv_heads * pl.head_groups *
+                            std::max(1, (max_kv_len + kKv4Tile - 1) / kKv4Tile);
+    pl.deep = tiles <= 11LL * st->sm_count;
+    int* occ = &st->kv4_occ[(head_dim == 64 ? 0 : 4) + (pl.nt - 1) * 2 + (pl.deep ? 1 : 0)];
+    int rc = kv4_dispatch(head_dim, pl.nt, pl.deep,
+                          [&](auto format) { return prepare_cached<decltype(format)>(occ); });
+    if (rc != FR_OK) return rc;
+    pl.ctas = (int)std::max<long long>(1, std::min<long long>((long long)st->sm_count * *occ, tiles));
+    pl.ws_bytes = kCounterBytes + (size_t)2 * pl.ctas * 8 * pl.nt * (head_dim + 2) * sizeof(float);
+    *out = pl;
+    return FR_OK;
+}
+
+int run_kv4(const void* q, long long q_stride, const fr_kv4_cache* cache, const int* block_table,
+            const int* kv_lens, void* out, int batch, int num_heads, int max_blocks,
+            int max_kv_len, cudaStream_t s) {
+    DeviceState* st = nullptr;
+    int rc = get_state(&st);
+    if (rc != FR_OK) return rc;
+    const int Hkv = cache->num_kv_heads, D = cache->head_dim;
+    CachedPlan pl;
+    rc = kv4_plan(st, batch, num_heads, Hkv, D, std::max(1, max_kv_len), &pl);
+    if (rc != FR_OK) return rc;
+    rc = ensure_workspace(st, pl.ws_bytes, s);
+    if (rc != FR_OK) return rc;
+    fr::CachedDecodeParams<fr::Kv4View> p;
+    std::memset(&p, 0, sizeof(p));
+    p.cache = kv4_view(cache);
+    p.q_stride = q_stride;
+    p.H = num_heads;
+    p.G = num_heads / Hkv;
+    p.head_groups = pl.head_groups;
+    p.bt_stride = max_blocks;
+    p.max_len = max_kv_len;
+    p.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)D));
+    p.counters = static_cast<int*>(st->ws);
+    p.max_units = kCachedUnits;
+    p.part_ml = reinterpret_cast<float*>(static_cast<char*>(st->ws) + kCounterBytes);
+    p.part_acc = p.part_ml + (size_t)2 * pl.ctas * 8 * pl.nt * 2;
+    p.min_tiles_per_cta = 2;
+    p.min_ctas = st->sm_count;
+    p.item_cost = 1;
+    p.merge_cost = 1;
+    p.whole_tiles = 3;
+    for (int b = 0; b < batch; b += pl.chunk) {
+        p.batch = std::min(pl.chunk, batch - b);
+        p.q = static_cast<const __half*>(q) + (size_t)b * q_stride;
+        p.out = static_cast<__half*>(out) + (size_t)b * num_heads * D;
+        p.kv_lens = kv_lens + b;
+        p.block_table = block_table + (size_t)b * max_blocks;
+        rc = kv4_dispatch(D, pl.nt, pl.deep,
+                          [&](auto format) { return launch_cached<decltype(format)>(p, pl.ctas, s); });
+        if (rc != FR_OK) return rc;
+    }
+    return FR_OK;
+}
+
+// Checks and lays out what both appends take; the pages are the caller's.
+int fill_append(const void* q, const void* k, const void* v, void* q_out, void* k_out, void* v_out,
+                const long long* token_strides, const void* q_bias, const void* k_bias,
+                const void* v_bias, const float* cos_tab, const float* sin_tab, int table_rows,
+                const int* positions, int num_axes, const unsigned char* freq_axis,
+                const long long* slots, int num_tokens, int num_heads, int num_kv_heads,
+                int head_dim, fr::PagedAppendParams* out) {
+    if (!q || !k || !v || !q_out || !cos_tab || !sin_tab || !positions || !slots ||
+        table_rows <= 0 || num_tokens < 0 || num_axes < 1 || num_axes > fr::kPagedAxes ||
+        (num_axes > 1 && !freq_axis))
+        return FR_ERR_INVALID_ARG;
+    int rc = check_heads(num_heads, num_kv_heads, head_dim);
+    if (rc != FR_OK) return rc;
+    fr::PagedAppendParams p;
+    std::memset(&p, 0, sizeof(p));
+    if (num_axes > 1)
+        for (int f = 0; f < head_dim / 2; ++f) {
+            if (freq_axis[f] >= num_axes) return FR_ERR_INVALID_ARG;
+            p.axis[f] = freq_axis[f];
+        }
+    p.by_eights = 1;
+    for (int f = 0; f < head_dim / 2; ++f) p.by_eights &= p.axis[f] == p.axis[f & ~7];
+    const long long heads[6] = {num_heads, num_kv_heads, num_kv_heads,
+                                num_heads, num_kv_heads, num_kv_heads};
+    const void* const in[3] = {q, k, v};
+    void* const outs[3] = {q_out, k_out, v_out};
+    const void* const bias[3] = {q_bias, k_bias, v_bias};
+    for (int i = 0; i < 6; ++i) {
+        p.stride[i] = token_strides ? token_strides[i] : heads[i] * head_dim;
+        const bool used = i < 3 || outs[i - 3];
+        if (used && (p.stride[i] < heads[i] * head_dim || p.stride[i] >= (1LL << 32)))
+            return FR_ERR_INVALID_ARG;
+        if (used && (p.stride[i] & 7)) return FR_ERR_MISALIGNED;
+    }
+    for (int i = 0; i < 3; ++i) {
+        // An output over its input has to lie as the input does.
+        if (outs[i] == in[i] && p.stride[3 + i] != p.stride[i]) return FR_ERR_INVALID_ARG;
+        if (!aligned(in[i], 16) || !aligned(outs[i], 16) || !aligned(bias[i], 16))
+            return FR_ERR_MISALIGNED;
+        p.in[i] = static_cast<const __half*>(in[i]);
+        p.out[i] = static_cast<__half*>(outs[i]);
+        p.bias[i] = static_cast<const __half*>(bias[i]);
+    }
+    if (!aligned(cos_tab, 16) || !aligned(sin_tab, 16) || !aligned(positions, 4) ||
+        !aligned(slots, 8))
+        return FR_ERR_MISALIGNED;
+    p.cos_tab = cos_tab;
+    p.sin_tab = sin_tab;
+    p.positions = positions;
+    p.slots = slots;
+    p.T = num_tokens;
+    p.H = num_heads;
+    p.Hkv = num_kv_heads;
+    p.table_rows = table_rows;
+    *out = p;
+    return FR_OK;
+}
+
+template <class Pages>
+int run_append(fr::PagedAppendParams p, int head_dim, cudaStream_t s) {
+    DeviceState* st = nullptr;
+    int rc = get_state(&st);
+    if (rc != FR_OK) return rc;
+    p.err = st->err;
+    const long long rows = fr::kPagedThreads / (head_dim / 16);             // of a CTA
+    const long long kv = (long long)p.T * p.Hkv;
+    const long long kv_ctas = (kv + rows - 1) / rows;
+    const long long q_rows = (long long)p.T * ((p.H + fr::kQRows - 1) / fr::kQRows);
+    const long long grid = 2 * kv_ctas + (q_rows + rows - 1) / rows;
+    if (kv + rows >= (1LL << 31) || grid >= (1LL << 31)) return FR_ERR_INVALID_ARG;
+    p.kv_ctas = (int)kv_ctas;
+    auto fn = head_dim == 64 ? fr::paged_append_kernel<64, Pages> : fr::paged_append_kernel<128, Pages>;
+    return launch_plain(fn, (unsigned)grid, fr::kPagedThreads, 0, s,
+                        static_cast<const fr::PagedAppendParams>(p));
+}
+
+}  // namespace
+
+extern "C" {
+
+int fr_qkv_rope_append_paged(const void* q, const void* k, const void* v, void* q_out, void* k_out,
+                             void* v_out, const long long* token_strides, const void* q_bias,
+                             const void* k_bias, const void* v_bias, const float* cos_tab,
+                             const float* sin_tab, int table_rows, const int* positions,
+                             int num_axes, const unsigned char* freq_axis, const long long* slots,
+                             void* k_pages, void* v_pages, int page_size, int num_pages,
+                             int num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                             void* stream) {
+    if (!k_pages || !v_pages || page_size <= 0 || page_size % kPageRows != 0 || num_pages <= 0)
+        return FR_ERR_INVALID_ARG;
+    fr::PagedAppendParams p;
+    int rc = fill_append(q, k, v, q_out, k_out, v_out, token_strides, q_bias, k_bias, v_bias, cos_tab,
+                         sin_tab, table_rows, positions, num_axes, freq_axis, slots, num_tokens,
+                         num_heads, num_kv_heads, head_dim, &p);
+    if (rc != FR_OK) return rc;
+    if (!aligned(k_pages, 16) || !aligned(v_pages, 16)) return FR_ERR_MISALIGNED;
+    if (num_tokens == 0) return FR_OK;
+    p.pages[0] = static_cast<__half*>(k_pages);
+    p.pages[1] = static_cast<__half*>(v_pages);
+    p.pool = (long long)num_pages * page_size;
+    return guarded([&]() -> int {
+        return run_append<fr::HalfPages>(p, head_dim, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int fr_qkv_rope_append_kv4(const void* q, const void* k, const void* v, void* q_out, void* k_out,
+                           void* v_out, const long long* token_strides, const void* q_bias,
+                           const void* k_bias, const void* v_bias, const float* cos_tab,
+                           const float* sin_tab, int table_rows, const int* positions,
+                           int num_axes, const unsigned char* freq_axis, const long long* slots,
+                           const fr_kv4_cache* cache, int num_tokens, int num_heads,
+                           void* stream) {
+    int rc = check_kv4(cache);
+    if (rc != FR_OK) return rc;
+    fr::PagedAppendParams p;
+    rc = fill_append(q, k, v, q_out, k_out, v_out, token_strides, q_bias, k_bias, v_bias, cos_tab,
+                     sin_tab, table_rows, positions, num_axes, freq_axis, slots, num_tokens,
+                     num_heads, cache->num_kv_heads, cache->head_dim, &p);
+    if (rc != FR_OK) return rc;
+    if (num_tokens == 0) return FR_OK;
+    p.cache = kv4_view(cache);
+    p.pool = (long long)cache->num_pages * cache->page_size;
+    return guarded([&]() -> int {
+        return run_append<fr::Kv4Pages>(p, cache->head_dim, static_cast<cudaStream_t>(stream));
+    });
+}
+
+int fr_kv4_gather(const fr_kv4_cache* cache, const long long* slots, void* k_out, void* v_out,
+                  int num_slots, void* stream) {
+    if (!slots || (!k_out && !v_out) || num_slots < 0) return FR_ERR_INVALID_ARG;
+    int rc = check_kv4(cache);
+    if (rc != FR_OK) return rc;
+    if (!aligned(slots, 8) || !aligned(k_out, 16) || !aligned(v_out, 16)) return FR_ERR_MISALIGNED;
+    if (num_slots == 0) return FR_OK;
+    return guarded([&]() -> int {
+        fr::Kv4GatherParams p;
+        p.cache = kv4_view(cache);
+        p.slots = slots;
+        p.k_out = static_cast<__half*>(k_out);
+        p.v_out = static_cast<__half*>(v_out);
+        p.pieces = (long long)num_slots * cache->num_kv_heads * (cache->head_dim / 16);
+        const long long grid = (p.pieces + 255) / 256;
+        if (grid >= (1LL << 31)) return FR_ERR_INVALID_ARG;
+        cudaStream_t s = static_cast<cudaStream_t>(stream);
+        auto fn = cache->head_dim == 64 ? fr::kv4_gather_kernel<64> : fr::kv4_gather_kernel<128>;
+        return launch_plain(fn, (unsigned)grid, 256, 0, s, static_cast<const fr::Kv4GatherParams>(p));
+    });
+}
+
+int fr_decode_attn_paged_kv4(const void* q, long long q_stride, const fr_kv4_cache* cache,
+                             const int* block_table, const int* kv_lens, void* out, int batch,
+                             int num_heads, int max_blocks_per_seq, int max_kv_len,
+                             void* stream) {
+    if (!q || !block_table || !kv_lens || !out || batch <= 0 || max_blocks_per_seq <= 0 ||
+        max_kv_len < 0 || max_kv_len >= (1 << 30))
+        return FR_ERR_INVALID_ARG;
+    int rc = check_kv4(cache);
+    if (rc != FR_OK) return rc;
+    if ((long long)max_blocks_per_seq * cache->page_size < max_kv_len) return FR_ERR_INVALID_ARG;
+    rc = check_heads(num_heads, cache->num_kv_heads, cache->head_dim);
+    if (rc != FR_OK) return rc;
+    const long long row = (long long)num_heads * cache->head_dim;
+    if (q_stride == 0) q_stride = row;
+    if (q_stride < row) return FR_ERR_INVALID_ARG;
+    if (!aligned(q, 16) || !aligned(out, 16) || (q_stride & 7) || !aligned(block_table, 4) ||
+        !aligned(kv_lens, 4))
+        return FR_ERR_MISALIGNED;
+    return guarded([&]() -> int {
+        return run_kv4(q, q_stride, cache, block_table, kv_lens, out, batch, num_heads,
+                       max_blocks_per_seq, max_kv_len, static_cast<cudaStream_t>(stream));
+    });
+}
+
+size_t fr_kv4_workspace_size(int batch, int num_heads, int num_kv_heads, int head_dim,
+                             int max_kv_len) {
+    if (batch <= 0 || max_kv_len < 0 || check_heads(num_heads, num_kv_heads, head_dim) != FR_OK)
+        return 0;
+    size_t bytes = 0;
+    guarded([&]() -> int {
+        DeviceState* st = nullptr;
+        CachedPlan pl;
+        int rc = get_state(&st);
+        if (rc == FR_OK)
+            rc = kv4_plan(st, batch, num_heads, num_kv_heads, head_dim, std::max(1, max_kv_len), &pl);
+        if (rc == FR_OK) bytes = pl.ws_bytes;
+        return rc;
+    });
+    return bytes;
+}
+
+}  // extern "C"

@@ -1,0 +1,375 @@
+// paged_append_kernels.cuh - decode/prefill prologue of the paged caches whose
+// rows stand by themselves, 16-bit pages and 4 bits: q/k/v bias + RoPE (one or
+// several position axes) + append through a slot map, in one launch; and the
+// read-back of 4-bit slots as fp16.
+//
+// Mathematics, per token t (all in fp32, one rounding at each output):
+//   x = x + bias;  for f < D/2 the pair (x[f], x[f + D/2]) of q and k turns to
+//   (a*c - b*s, a*s + b*c) with c, s = tables[positions[axis(f)][t]][f].
+// In 4 bits, per group of 64 dims of a row of K or V:
+//   bias  = min x rounded down to fp16
+//   scale = (max x - bias) / 15 rounded up to fp16
+//   code  = round((x - bias) / scale), ties to even (0 where scale is 0)
+// so every quotient lies in 0 .. 15 and a value is off by half a scale at most.
+// A group with a NaN, an infinity or a minimum below fp16's range gets a NaN
+// scale and bias and reads back as NaN.
+//
+// Layout: LPR = D / 16 lanes share a row, lane l holding the pairs f = 8l ..
+// 8l + 7, so that rows move in 16-byte accesses and a lane's codes are two whole
+// words.  No row depends on another: CTAs take rows of K, of V, and of q (kQRows
+// heads of a token to a lane group, which looks the angles up once).
+#pragma once
+#include "fr_ptx.cuh"
+#include "kv4_common.cuh"
+#include <cstdint>
+
+namespace fr {
+
+constexpr int kPagedThreads = 128;
+constexpr int kPagedAxes = 4;
+constexpr int kQRows = 4;               // query rows that a lane group has under way
+
+struct PagedAppendParams {
+    const __half* in[3];                // q, k, v
+    __half* out[3];                     // k's, v's: nullptr = not written
+    long long stride[6];                // halves between tokens: q, k, v, then the outputs
+    const __half* bias[3];
+    const float* cos_tab;
+    const float* sin_tab;
+    const int* positions;               // [axes][T]
+    const long long* slots;
+    __half* pages[2];                   // 16-bit: K's, V's rows [slots][Hkv][D]
+    Kv4View cache;                      // 4 bits
+    long long pool;                     // slots
+    int* err;
+    int T, H, Hkv, table_rows;
+    int by_eights;                      // every group of eight frequencies has one axis
+    int kv_ctas;                        // of K; as many of V
+    uint8_t axis[64];                   // axis of frequency f
+};
+
+// Sixteen values of a row: its pairs 8l .. 8l + 7 (first halves, second halves).
+struct Row16 {
+    float lo[8], hi[8];
+};
+
+__device__ __forceinline__ void unpack8(uint4 w, float (&x)[8]) {
+    const uint32_t h[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+    return make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]),
+                      pack_half2(x[6], x[7]));
+}
+
+template <int D>
+__device__ __forceinline__ void store_row16(__half* row, int f0, const Row16& r) {
+    *reinterpret_cast<uint4*>(row + f0) = pack8(r.lo);
+    *reinterpret_cast<uint4*>(row + f0 + D / 2) = pack8(r.hi);
+}
+
+// Cosines and sines of token t at the lane's eight frequencies.  A position
+// outside the table is recorded and read as position 0.
+template <int D>
+__device__ __forceinline__ void load_angles(const PagedAppendParams& p, int t, int f0, float (&c)[8],
+                                            float (&s)[8]) {
+    constexpr int kHalf = D / 2;
+    auto at = [&](int axis) {
+        int pos = p.positions[(size_t)axis * p.T + t];
+        if ((unsigned)pos >= (unsigned)p.table_rows) {
+            record_error(p.err, kDevBadIndex);
+            pos = 0;
+        }
+        return pos;
+    };
+    if (p.by_eights) {
+        const size_t e = (size_t)at(p.axis[f0]) * kHalf + f0;
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+            const float4 cv = *reinterpret_cast<const float4*>(p.cos_tab + e + j);
+            const float4 sv = *reinterpret_cast<const float4*>(p.sin_tab + e + j);
+            c[j] = cv.x; c[j + 1] = cv.y; c[j + 2] = cv.z; c[j + 3] = cv.w;
+            s[j] = sv.x; s[j + 1] = sv.y; s[j + 2] = sv.z; s[j + 3] = sv.w;
+        }
+        return;
+    }
+#pragma unroll 1
+    for (int j = 0; j < 8; ++j) {
+        const size_t e = (size_t)at(p.axis[f0 + j]) * kHalf + f0 + j;
+        const float cj = p.cos_tab[e], sj = p.sin_tab[e];
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            if (x == j) { c[x] = cj; s[x] = sj; }
+    }
+}
+
+// The products are rounded before they are added, as separate operations
+// would: which codes a row gets does not hang on contraction.
+__device__ __forceinline__ void turn16(Row16& r, const float (&c)[8], const float (&s)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float a = r.lo[j], b = r.hi[j];
+        r.lo[j] = __fsub_rn(__fmul_rn(a, c[j]), __fmul_rn(b, s[j]));
+        r.hi[j] = __fadd_rn(__fmul_rn(a, s[j]), __fmul_rn(b, c[j]));
+    }
+}
+
+template <int D>
+__device__ __forceinline__ void add_bias16(Row16& r, const __half* bias, int f0) {
+    Row16 b;
+    unpack8(*reinterpret_cast<const uint4*>(bias + f0), b.lo);
+    unpack8(*reinterpret_cast<const uint4*>(bias + f0 + D / 2), b.hi);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        r.lo[j] = __fadd_rn(r.lo[j], b.lo[j]);
+        r.hi[j] = __fadd_rn(r.hi[j], b.hi[j]);
+    }
+}
+
+// ---------------------------------------------------------------- 16-bit pages
+struct HalfPages {
+    template <int D>
+    static __device__ __forceinline__ void put(const PagedAppendParams& p, int which, int h, long long slot,
+                                               int f0, const Row16& r, bool real) {
+        if (real) store_row16<D>(p.pages[which] + (slot * p.Hkv + h) * D, f0, r);
+    }
+};
+
+// --------------------------------------------------------------------- 4 bits
+// Minima and maxima that are NaN if an operand is.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+struct Kv4Pair {
+    float scale, bias, inverse;
+    __half2 bits;
+};
+
+// Scale and bias of a group whose least and largest values are low and high.
+__device__ __forceinline__ Kv4Pair kv4_pair(float low, float high) {
+    Kv4Pair r;
+    const __half b = __float2half_rd(__fadd_rn(low, 0.f));          // -0 is stored as 0
+    r.bias = __half2float(b);
+    const __half s = __float2half_ru(__fdiv_rn(__fsub_rn(high, r.bias), 15.f));
+    r.scale = __half2float(s);
+    r.bits = __halves2half2(s, b);
+    // not finite: an exponent of all ones in either
+    if (!(fabsf(r.bias) < INFINITY && r.scale < INFINITY)) {
+        r.scale = 0.f;
+        r.bits = __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0x7fff));
+    }
+    r.inverse = r.scale > 0.f ? __frcp_rn(r.scale) : 0.f;
+    return r;
+}
+
+// Codes of eight values.  The quotient is rounded as the division itself would:
+// q0 = x * (1 / scale), then one correction by the exact remainder (Markstein's
+// theorem: correctly rounded when the reciprocal is).  y + 1.5 * 2^23 is rounded
+// to a whole number, whose low bits are the code.  The codes of a group that is
+// not finite are 0 (inverse 0; NaN and infinity times 0 are not whole numbers).
+__device__ __forceinline__ uint32_t kv4_codes(const float (&x)[8], const Kv4Pair& g) {
+    uint32_t n[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float d = __fsub_rn(x[j], g.bias);
+        const float q0 = __fmul_rn(d, g.inverse);
+        const float y = __fmaf_rn(__fmaf_rn(-q0, g.scale, d), g.inverse, q0);
+        n[j] = __float_as_uint(__fadd_rn(y, 12582912.f));
+    }
+    uint32_t two[4];                            // low byte: two codes
+#pragma unroll
+    for (int j = 0; j < 4; ++j) two[j] = (n[2 * j] & 15u) | (n[2 * j + 1] << 4);
+    const uint32_t w = __byte_perm(__byte_perm(two[0], two[1], 0x0040),
+                                   __byte_perm(two[2], two[3], 0x0040), 0x5410);
+    return g.inverse > 0.f ? w : 0u;
+}
+
+struct Kv4Pages {
+    // Every lane of the row takes part, also where the row is not cached.
+    template <int D>
+    static __device__ __forceinline__ void put(const PagedAppendParams& p, int which, int h, long long slot,
+                                               int f0, const Row16& r, bool real) {
+        constexpr int NG = D / kKv4Group, LPR = D / 16;
+        float low[2], high[2];                  // of the first halves, of the second
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const float (&v)[8] = x ? r.hi : r.lo;
+            low[x] = high[x] = v[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) {
+                low[x] = min_nan(low[x], v[j]);
+                high[x] = max_nan(high[x], v[j]);
+            }
+        }
+        if (NG == 1) {
+            low[0] = min_nan(low[0], low[1]);
+            high[0] = max_nan(high[0], high[1]);
+        }
+        Kv4Pair g[NG];
+#pragma unroll
+        for (int x = 0; x < NG; ++x) {
+#pragma unroll
+            for (int o = 1; o < LPR; o <<= 1) {
+                low[x] = min_nan(low[x], __shfl_xor_sync(0xffffffffu, low[x], o));
+                high[x] = max_nan(high[x], __shfl_xor_sync(0xffffffffu, high[x], o));
+            }
+            g[x] = kv4_pair(low[x], high[x]);
+        }
+        if (!real) return;
+        const Kv4View& c = p.cache;
+        const int page = int(slot / c.page_size), row = int(slot - (long long)page * c.page_size);
+        uint8_t* dst = (which ? c.v : c.k) + c.row(page, h, row) + f0 / 2;
+        *reinterpret_cast<uint32_t*>(dst) = kv4_codes(r.lo, g[0]);
+        *reinterpret_cast<uint32_t*>(dst + D / 4) = kv4_codes(r.hi, g[NG - 1]);
+        __half2* pairs = c.pairs<D>(page, h, row) + which * NG;
+        if (f0 == 0) {
+#pragma unroll
+            for (int x = 0; x < NG; ++x) pairs[x] = g[x].bits;
+        }
+    }
+};
+
+// CTAs 0 .. kv_ctas - 1: rows of K (a lane group per token and kv head); as
+// many: of V; the others: kQRows query heads of a token per lane group.
+template <int D, class Pages>
+__global__ void __launch_bounds__(kPagedThreads)
+paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
+    constexpr int LPR = D / 16;
+    constexpr int ROWS = kPagedThreads / LPR;
+    const int f0 = (threadIdx.x % LPR) * 8;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    if (blockIdx.x < 2 * p.kv_ctas) {
+        const int which = blockIdx.x >= p.kv_ctas;
+        const int i = (blockIdx.x - which * p.kv_ctas) * ROWS + threadIdx.x / LPR;
+        const bool there = i < p.T * p.Hkv;
+        const int t = there ? i / p.Hkv : 0, h = i - t * p.Hkv;
+        long long slot = -1;
+        uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if (there) {
+            const __half* src = p.in[1 + which] + t * p.stride[1 + which] + (size_t)h * D + f0;
+            raw[0] = *reinterpret_cast<const uint4*>(src);
+            raw[1] = *reinterpret_cast<const uint4*>(src + D / 2);
+            slot = p.slots[t];
+        }
+        const bool held = slot >= 0 && slot < p.pool;
+        Row16 r;
+        unpack8(raw[0], r.lo);
+        unpack8(raw[1], r.hi);
+        if (slot >= 0) {
+            if (!held && h == 0 && f0 == 0) record_error(p.err, kDevBadIndex);
+            if (p.bias[1 + which]) add_bias16<D>(r, p.bias[1 + which] + (size_t)h * D, f0);
+            if (!which) {
+                float c[8], s[8];
+                load_angles<D>(p, t, f0, c, s);
+                turn16(r, c, s);
+            }
+            if (p.out[1 + which])
+                store_row16<D>(p.out[1 + which] + t * p.stride[4 + which] + (size_t)h * D, f0, r);
+        }
+        Pages::template put<D>(p, which, h, slot, f0, r, held);
+        return;
+    }
+    const int chunks = (p.H + kQRows - 1) / kQRows;
+    const long long i = (long long)(blockIdx.x - 2 * p.kv_ctas) * ROWS + threadIdx.x / LPR;
+    if (i >= (long long)p.T * chunks) return;
+    const int t = int(i / chunks);
+    const int h0 = int(i - (long long)t * chunks) * kQRows;
+    const __half* src = p.in[0] + t * p.stride[0] + (size_t)h0 * D + f0;
+    // The rows are on their way before the slot tells whether the token takes part.
+    uint4 raw[kQRows][2];
+#pragma unroll
+    for (int j = 0; j < kQRows; ++j)
+        if (h0 + j < p.H) {
+            raw[j][0] = *reinterpret_cast<const uint4*>(src + j * D);
+            raw[j][1] = *reinterpret_cast<const uint4*>(src + j * D + D / 2);
+        }
+    if (p.slots[t] < 0) return;
+    float c[8], s[8];
+    load_angles<D>(p, t, f0, c, s);
+    __half* dst = p.out[0] + t * p.stride[3] + (size_t)h0 * D;
+#pragma unroll
+    for (int j = 0; j < kQRows; ++j)
+        if (h0 + j < p.H) {
+            Row16 r;
+            unpack8(raw[j][0], r.lo);
+            unpack8(raw[j][1], r.hi);
+            if (p.bias[0]) add_bias16<D>(r, p.bias[0] + (size_t)(h0 + j) * D, f0);
+            turn16(r, c, s);
+            store_row16<D>(dst + j * D, f0, r);
+        }
+}
+
+// ---------------------------------------------------------------------------
+// Read-back: out[i] = fp16(code * scale + bias) of slot slots[i], every kv head;
+// a slot outside the pool gives zeros.  One thread widens 16 codes (an 8-byte
+// load) of K and of V, into 32 bytes each.
+// ---------------------------------------------------------------------------
+struct Kv4GatherParams {
+    Kv4View cache;
+    const long long* slots;
+    __half* k_out;
+    __half* v_out;
+    long long pieces;                   // slots x Hkv x D / 16
+};
+
+__device__ __forceinline__ void kv4_widen16(uint2 w, __half2 pair, __half* out) {
+    const float2 g = __half22float2(pair);
+    const uint32_t in[2] = {w.x, w.y};
+    uint4 h[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = fmaf(float((in[i] >> (4 * j)) & 15u), g.x, g.y);
+        h[i] = pack8(x);
+    }
+    reinterpret_cast<uint4*>(out)[0] = h[0];
+    reinterpret_cast<uint4*>(out)[1] = h[1];
+}
+
+template <int D>
+__global__ void __launch_bounds__(256)
+kv4_gather_kernel(const Kv4GatherParams p) {
+    constexpr int PPR = D / 16;                 // pieces per row
+    constexpr int NG = D / kKv4Group;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= p.pieces) return;
+    const Kv4View& c = p.cache;
+    const int e = int(i % PPR) * 16;
+    const long long row = i / PPR;
+    const int h = int(row % c.Hkv);
+    const long long slot = p.slots[row / c.Hkv];
+    const bool real = slot >= 0 && slot < (long long)c.num_pages * c.page_size;
+    const int page = real ? int(slot / c.page_size) : 0;
+    const int r = real ? int(slot - (long long)page * c.page_size) : 0;
+    const __half2 zero = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
+    __half2 kp = zero, vp = zero;
+    uint2 kw = make_uint2(0, 0), vw = kw;
+    if (real) {
+        const size_t at = c.row(page, h, r) + e / 2;
+        const __half2* pairs = c.pairs<D>(page, h, r) + e / kKv4Group;
+        if (p.k_out) { kw = *reinterpret_cast<const uint2*>(c.k + at); kp = pairs[0]; }
+        if (p.v_out) { vw = *reinterpret_cast<const uint2*>(c.v + at); vp = pairs[NG]; }
+    }
+    if (p.k_out) kv4_widen16(kw, kp, p.k_out + row * D + e);
+    if (p.v_out) kv4_widen16(vw, vp, p.v_out + row * D + e);
+}
+
+}  // namespace fr

@@ -386,6 +386,98 @@ FR_API int fr_decode_attn_paged_kv8(const void* q, long long q_stride, const fr_
 FR_API size_t fr_kv8_workspace_size(int batch, int num_heads, int num_kv_heads, int head_dim,
                                     int max_kv_len);
 
+/* Prologue of the 16-bit paged cache (the pages that fr_decode_attn_paged
+ * reads), one launch: q/k/v bias, NeoX RoPE on q and k, K and V written to the
+ * pages at the tokens' slots (fr_paged_step's).  All arithmetic in fp32; the
+ * cached rows, q_out, k_out and v_out are rounded to fp16 once.
+ *   k_pages, v_pages  [num_pages, page_size, num_kv_heads, head_dim] fp16; slot
+ *               s is row s % page_size of page s / page_size, page_size a
+ *               multiple of 16
+ * The other arguments are fr_qkv_rope_append_kv8's, with these differences:
+ * q, k, v, their outputs, biases and pages are 16-byte aligned and
+ * token_strides multiples of 8.  A token whose slot is negative is left out; a
+ * position outside the table (read as 0) or a slot past the pool (not cached;
+ * the token's outputs are written) is recorded in the error word.  The slots of
+ * a call differ from one another (negative ones aside). */
+FR_API int fr_qkv_rope_append_paged(const void* q, const void* k, const void* v, void* q_out,
+                                    void* k_out, void* v_out, const long long* token_strides,
+                                    const void* q_bias, const void* k_bias, const void* v_bias,
+                                    const float* cos_tab, const float* sin_tab, int table_rows,
+                                    const int* positions, int num_axes,
+                                    const unsigned char* freq_axis, const long long* slots,
+                                    void* k_pages, void* v_pages, int page_size, int num_pages,
+                                    int num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                                    void* stream);
+
+/* ---- Serving from a paged cache held in 4 bits ---------------------------
+ * As with the 8-bit cache: fr_paged_step, then per layer
+ * fr_qkv_rope_append_kv4 and fr_decode_attn_paged_kv4, on one stream and
+ * capturable in a CUDA graph.  No reference counterpart.
+ *
+ * A row (one token, one kv head) of K or V is held in groups of FR_KV4_GROUP
+ * dims, each with a scale and a bias: a cached value is code * scale + bias,
+ * codes 0 .. 15, two to a byte (dim 2i in the low half of byte i, dim 2i + 1 in
+ * the high half).  k and v hold the codes of
+ * [num_pages][num_kv_heads][page_size][head_dim / 2 bytes]; the last dimension
+ * is contiguous, the others have the strides given (in bytes, multiples of 16).
+ *   scales [num_pages][num_kv_heads][page_size][2 (K, V)][head_dim / FR_KV4_GROUP]
+ *          [2 (scale, bias)] fp16, finite, scales not negative
+ * Slot s is row s % page_size of page s / page_size. */
+#define FR_KV4_GROUP 64
+
+typedef struct fr_kv4_cache {
+    void* k;                   /* 16-byte aligned */
+    void* v;
+    void* scales;              /* 16-byte aligned */
+    int num_pages;
+    int page_size;             /* a multiple of 16 rows */
+    int num_kv_heads;
+    int head_dim;              /* 64 or 128 */
+    long long page_stride;     /* bytes between pages, kv heads and rows */
+    long long head_stride;
+    long long row_stride;
+} fr_kv4_cache;
+
+/* Prologue of the 4-bit cache, one launch; fr_qkv_rope_append_paged's arguments.
+ * Codes: per row of K (turned) or V and group of dims, in fp32,
+ *   bias  = the largest fp16 number not above the group's minimum
+ *   scale = the smallest fp16 number not below (maximum - bias) / 15
+ *   code  = (x - bias) / scale to the nearest, ties to even (0 if scale is 0)
+ * so that no value is cut off and each is off by half a scale at most.  A group
+ * that holds a NaN, an infinity or a value below -65504 gets NaN for both and
+ * reads back as NaN; no row's codes depend on another row. */
+FR_API int fr_qkv_rope_append_kv4(const void* q, const void* k, const void* v, void* q_out,
+                                  void* k_out, void* v_out, const long long* token_strides,
+                                  const void* q_bias, const void* k_bias, const void* v_bias,
+                                  const float* cos_tab, const float* sin_tab, int table_rows,
+                                  const int* positions, int num_axes,
+                                  const unsigned char* freq_axis, const long long* slots,
+                                  const fr_kv4_cache* cache, int num_tokens, int num_heads,
+                                  void* stream);
+
+/* Reads slots back as fp16: k_out, v_out [num_slots, num_kv_heads, head_dim]
+ * (16-byte aligned; either may be NULL).  A slot outside the pool gives zeros. */
+FR_API int fr_kv4_gather(const fr_kv4_cache* cache, const long long* slots, void* k_out,
+                         void* v_out, int num_slots, void* stream);
+
+/* Decode attention over the 4-bit paged cache, one token per sequence;
+ * fr_decode_attn_paged_kv8's arguments.  Rows past a sequence's end are never
+ * used, whatever they hold.  A NaN scale or bias of a used row makes the outputs
+ * it enters NaN.  Scores and sums are fp32.  A short call is off by the rounding
+ * of its outputs; a long one also rounds each weight (a probability times V's
+ * scale) to fp16, 2^-11 of itself, which counts by the value's distance from
+ * code 8.  A call is long when batch * num_kv_heads sequences of max_kv_len, in
+ * tiles of 128 positions (once more for each 16 query heads of a group above
+ * 16), make more than 11 tiles per SM, at most 512 sequences counted.  The
+ * result does not depend on which CTA merges: equal inputs give equal bits. */
+FR_API int fr_decode_attn_paged_kv4(const void* q, long long q_stride, const fr_kv4_cache* cache,
+                                    const int* block_table, const int* kv_lens, void* out,
+                                    int batch, int num_heads, int max_blocks_per_seq,
+                                    int max_kv_len, void* stream);
+/* Workspace bytes one such call uses (see fr_reserve_workspace). */
+FR_API size_t fr_kv4_workspace_size(int batch, int num_heads, int num_kv_heads, int head_dim,
+                                    int max_kv_len);
+
 /* Grows the current device's workspace to at least `bytes` (call before
  * CUDA-graph capture).  fr_decode_workspace_size() gives the bytes one call
  * of fr_decode_attn_batched with these sizes needs (fr_decode_attn: batch 1). */
@@ -402,7 +494,7 @@ FR_API size_t fr_prefill_workspace_size(int seq_len, int num_heads, int head_dim
 
 /* Reads (and optionally clears) the current device's in-kernel error words
  * (the regular entry points' and fr_decode_attn_noalloc's): 0 = none,
- * 4 = an index out of range (fr_qkv_rope_append_kv8; FR_ERR_INVALID_ARG is
+ * 4 = an index out of range (the paged appends; FR_ERR_INVALID_ARG is
  * returned), otherwise a bounded wait ran out (FR_ERR_TIMEOUT is returned,
  * also when an index was out of range before or after).  Synchronises the
  * device; creates no state and allocates nothing. */
