@@ -20,8 +20,7 @@
 //   Query, State   q in registers; the running (m, l, o) of an item
 //   consume        one step
 //   dim(dm, g)     first of the two dims that lane group g holds in fragment
-//                  dm of o; four neighbouring dm from a multiple of four on
-//                  are eight consecutive dims
+//                  dm of o; kRun (4 or 1) neighbouring dm are consecutive dims
 #pragma once
 #include "batched_kernels.cuh"
 
@@ -298,7 +297,7 @@ cached_decode_kernel(const __grid_constant__ typename F::Params p) {
             const uint32_t kst = ring + ls * (2 * S::kStepBytes);
             load.copy(p, kst, kst + S::kStepBytes, scales_s + ls * S::kStepScales,
                       hg == 1 ? load.cur.j : load.cur.j / hg, lane, policy);
-            load.advance(seq_start, B, upb);
+            load.advance(p, seq_start, lens, B, upb, warp, lane);
             if (++lk < n) load.look_up(p, lens, warp);
             ls = ls + 1 == STAGES ? 0 : ls + 1;
         }
@@ -321,16 +320,17 @@ cached_decode_kernel(const __grid_constant__ typename F::Params p) {
         const size_t head_base = (size_t)b * p.H + h0;
 
         typename F::Query q;
-        q.load(p.q + (size_t)b * p.q_stride + (size_t)h0 * D, gcount, lane);
+        q.load(p.q + (size_t)b * p.q_stride + (size_t)h0 * D, gcount, sl2, lane);
         typename F::State st;
         st.clear();
-        for (int tt = 0; tt < cnt; ++tt, ++k) {
+        int valid = len - (i0 * NW + warp) * (16 * MT);     // positions from the warp's step on
+        const int k_end = k + cnt;
+        for (; k < k_end; ++k, valid -= TILE) {
             __syncwarp();                       // the stage refilled now is read by every lane
             start_step();
             cp_async_wait<STAGES - 1>();
             __syncwarp();                       // every lane's copies have landed
             const uint32_t kst = ring + stage * (2 * S::kStepBytes);
-            const int valid = len - ((i0 + tt) * NW + warp) * (16 * MT);
             if (valid > 0)
                 F::consume(kst, kst + S::kStepBytes, scales + stage * S::kStepScales, valid, q, st, sl2, lane);
             stage = stage + 1 == STAGES ? 0 : stage + 1;
@@ -369,12 +369,15 @@ cached_decode_kernel(const __grid_constant__ typename F::Params p) {
                         if (hj < gcount) {
                             __half* dst = p.out + (head_base + hj) * D;
 #pragma unroll
-                            for (int dm = 0; dm < DTILES; dm += 4) {
-                                uint32_t h[4];
+                            for (int dm = 0; dm < DTILES; dm += F::kRun) {
+                                uint32_t h[F::kRun];
 #pragma unroll
-                                for (int x = 0; x < 4; ++x)
+                                for (int x = 0; x < F::kRun; ++x)
                                     h[x] = pack_half2(st.o[dm + x][nt][jj] * inv, st.o[dm + x][nt][jj + 2] * inv);
-                                *reinterpret_cast<uint4*>(dst + F::dim(dm, g)) = make_uint4(h[0], h[1], h[2], h[3]);
+                                if constexpr (F::kRun == 4)
+                                    *reinterpret_cast<uint4*>(dst + F::dim(dm, g)) = make_uint4(h[0], h[1], h[2], h[3]);
+                                else
+                                    *reinterpret_cast<uint32_t*>(dst + F::dim(dm, g)) = h[0];
                             }
                         }
                     }

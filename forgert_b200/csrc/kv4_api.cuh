@@ -12,9 +12,17 @@ int check_kv4(const fr_kv4_cache* c) {
         c->page_size % kPageRows != 0 || c->num_kv_heads <= 0)
         return FR_ERR_INVALID_ARG;
     if (c->head_dim != 64 && c->head_dim != 128) return FR_ERR_UNSUPPORTED;
-    const long long limit = 1LL << 40;
     for (long long s : {c->page_stride, c->head_stride, c->row_stride})
-        if (s < c->head_dim / 2 || s >= limit) return FR_ERR_INVALID_ARG;
+        if (s < c->head_dim / 2) return FR_ERR_INVALID_ARG;
+    // The decode kernel counts 16-byte pieces in 32 bits: codes of K (or V) and
+    // scales below 64 GB each.
+    const long long limit = 1LL << 32, pages = c->num_pages;
+    const long long scales = (long long)c->num_kv_heads * c->page_size * (c->head_dim / 8) / 16;
+    if (c->page_stride >= limit || c->head_stride >= limit * 16 / c->num_kv_heads ||
+        c->row_stride >= limit * 16 / c->page_size || scales >= limit / pages ||
+        pages * (c->page_stride / 16) + c->num_kv_heads * (c->head_stride / 16) +
+                c->page_size * (c->row_stride / 16) >= limit)
+        return FR_ERR_INVALID_ARG;
     if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(c->scales, 16) ||
         ((c->page_stride | c->head_stride | c->row_stride) & 15))
         return FR_ERR_MISALIGNED;
@@ -32,21 +40,28 @@ fr::Kv4View kv4_view(const fr_kv4_cache* c) {
     v.page_stride = c->page_stride;
     v.head_stride = c->head_stride;
     v.row_stride = c->row_stride;
+    v.page16 = (uint32_t)(c->page_stride / 16);
+    v.block16 = (uint32_t)c->row_stride;
+    v.head_scales16 = (uint32_t)(c->page_size * (c->head_dim / 8) / 16);
+    v.scales16 = c->num_kv_heads * v.head_scales16;
     return v;
 }
 
-// Shapes of the decode kernel: four warps, steps of 32 rows.
-template <int D, int NT, bool DEEP> struct Kv4Shape;
+// Shapes of the decode kernel: four warps, kMT blocks of 16 rows a step (what a
+// step costs beside its blocks, about 86 instructions a warp, is a seventh of the
+// two blocks' at D = 128; at D = 64 four blocks a step instead of two, 32 sequences
+// of 8192 to 16384 tokens, 8 heads: 60.6 -> 54.7 us).
+//   for long calls three CTAs per SM (168 registers; at 128 for four the state
+//     spills: 64 sequences of 8192 to 32768 tokens 149 -> 246 us);
+//   DEEP, for calls of few tiles per SM: fewer CTAs, weights in two fp16 parts.
+template <int D, int NT, bool DEEP> struct Kv4Shape {
+    static constexpr int kMT = 2, kCtas = 2, kStages = 4;
+};
 template <> struct Kv4Shape<128, 1, false> { static constexpr int kMT = 2, kCtas = 3, kStages = 3; };
-template <> struct Kv4Shape<128, 1, true> { static constexpr int kMT = 2, kCtas = 2, kStages = 4; };
-template <> struct Kv4Shape<128, 2, false> { static constexpr int kMT = 2, kCtas = 2, kStages = 4; };
-template <> struct Kv4Shape<128, 2, true> { static constexpr int kMT = 2, kCtas = 2, kStages = 4; };
-template <> struct Kv4Shape<64, 1, false> { static constexpr int kMT = 2, kCtas = 4, kStages = 4; };
+template <> struct Kv4Shape<64, 1, false> { static constexpr int kMT = 4, kCtas = 3, kStages = 3; };
 template <> struct Kv4Shape<64, 1, true> { static constexpr int kMT = 2, kCtas = 3, kStages = 4; };
-template <> struct Kv4Shape<64, 2, false> { static constexpr int kMT = 2, kCtas = 2, kStages = 4; };
-template <> struct Kv4Shape<64, 2, true> { static constexpr int kMT = 2, kCtas = 2, kStages = 4; };
 constexpr int kKv4Warps = 4;
-constexpr int kKv4Tile = 16 * 2 * kKv4Warps;
+constexpr int kKv4Tile = 16 * 2 * kKv4Warps;    // the least of any shape: tiles of a call are at most as many
 
 template <int D, int NT, bool DEEP>
 using Kv4FormatOf = fr::Kv4Format<D, NT, Kv4Shape<D, NT, DEEP>::kMT, Kv4Shape<D, NT, DEEP>::kStages,
@@ -77,7 +92,7 @@ int kv4_plan(DeviceState* st, int batch, int num_heads, int num_kv_heads, int he
     if (pl.chunk <= 0) return FR_ERR_INVALID_ARG;
     const long long tiles = (long long)pl.chunk * num_kv_heads * pl.head_groups *
                             std::max(1, (max_kv_len + kKv4Tile - 1) / kKv4Tile);
-    pl.deep = tiles <= 11LL * st->sm_count;
+        pl.deep = tiles <= 11LL * st->sm_count;
     int* occ = &st->kv4_occ[(head_dim == 64 ? 0 : 4) + (pl.nt - 1) * 2 + (pl.deep ? 1 : 0)];
     int rc = kv4_dispatch(head_dim, pl.nt, pl.deep,
                           [&](auto format) { return prepare_cached<decltype(format)>(occ); });

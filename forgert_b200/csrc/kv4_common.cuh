@@ -21,6 +21,9 @@ struct Kv4View {
     __half* scales;
     int num_pages, page_size, Hkv;
     long long page_stride, head_stride, row_stride;   // bytes
+    // The same in numbers of 16 bytes, which fit 32 bits: a page, a block of 16
+    // rows; a page's scales, a head's part of them.
+    uint32_t page16, block16, scales16, head_scales16;
 
     __device__ __forceinline__ size_t row(int page, int head, int r) const {
         return (size_t)page * page_stride + (size_t)head * head_stride + (size_t)r * row_stride;

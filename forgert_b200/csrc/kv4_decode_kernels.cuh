@@ -14,43 +14,55 @@
 // bottom (half the error).  Scores, l, o and all other sums are fp32.
 //
 // A weight p a' enters the product with V as fp16 on a reference of its own
-// group's (r_g), 2^8 up, so that one as small as 2^-22 of the largest keeps all
-// its bits; REST adds a second product with what the rounding takes off (short
-// calls, where the outputs average fewer terms).  l and the middles are on the
-// first group's reference, in fp32 from unrounded p.
+// group's, 2^8 up, so that one as small as 2^-22 of the largest keeps all its
+// bits; REST adds a second product with what the rounding takes off (short calls,
+// where the outputs average fewer terms).  l and the middles are on the first
+// group's reference, in fp32 from unrounded p.
 //
 // Bytes: D of codes per position and kv head, D / 8 of scales; 4 * D * G
-// operations on them.
+// operations on them.  At D = 128 a block of 16 positions and one kv head takes a
+// warp about 287 instructions, 124 of them on the integer pipe, which takes one in
+// two cycles: 80 masks and shifts of codes (5 for 8 codes), 18 products.
 //
-// Fragments (mma m16n8k16), without ldmatrix: of K a lane holds 16 dims of each
-// group in two rows, of V eight dims (one word) of each group in four rows;
-// contraction order is free, so q is permuted to the order that masks bring K's
-// codes in (Kv4Query), and V's rows are paired by byte permutations.  Row i of a
-// block's fragments is row pos_of(i): rows two and four apart then differ mod 4,
-// which with the chunks exchanged by row (kv4_offset) keeps all loads from
-// shared memory free of bank conflicts.
+// Fragments (mma m16n8k16): of K a lane holds 16 dims of each group in rows 2g and
+// 2g + 1 of the block, as they lie in memory; contraction order is free, so q is
+// permuted to the order that masks bring K's codes in (Kv4Query).  V comes
+// transposed by bytes (ldmatrix m16n16 .trans .b8): four rows' bytes of one pair
+// of dims in a word, so that the same masks make (row, row + 2) operands of it.
 #pragma once
 #include "cached_decode_kernels.cuh"
 #include "kv4_common.cuh"
+#include <type_traits>
 
 namespace fr {
 
 constexpr float kKv4Shift = 8.f;        // a weight at its reference counts 2^8 ...
-constexpr float kKv4Top = 15.f;         // ... and may grow to 2^15 before that moves (fp16: < 2^16)
+constexpr float kKv4Most = 0x1p15f;     // ... and the weights of a lane's rows may sum up to 2^15 before that moves
 constexpr float kKv4Least = -24.f;      // a smaller scale's reference is this scale's: p stays below 2^39
+constexpr int kKv4Centre = 16;          // blocks between two subtractions of z
 constexpr uint32_t kLowHalves = 0x000f000fu, kHighHalves = 0x00f000f0u;
 
-__device__ __forceinline__ int kv4_pos_of(int i) { return i ^ ((i >> 2) & 1); }
-
-// Byte offset of byte b of row r in a step's K or V.
+// A block (16 rows) in shared memory: lines of 128 bytes, of 2 rows (D = 128) or 4,
+// as in the cache (copies that scatter a line's 32-byte sectors over lines took
+// 170 us where these take 155).  Within a line K's 32-byte half rows and V's
+// 16-byte chunks are exchanged by line, so that the loads of K (8 bytes of rows r,
+// r + 2, r + 4, r + 6 at a time) and V (16 bytes of 8 rows) hit distinct banks.
+template <int D> constexpr int kv4_block_bytes() { return 16 * (D / 2); }
+// 16-byte chunk c of row r.
 template <int D>
-__device__ __forceinline__ uint32_t kv4_offset(int r, int b) {
-    return D == 128 ? uint32_t(r * 64 + (b ^ ((r & 2) << 4))) : uint32_t(r * 32 + b);
+__device__ __forceinline__ uint32_t kv4_k_offset(int r, int c) {
+    return D == 128 ? r / 2 * 128 + ((r % 2 * 2 + c / 2) ^ (r / 2 % 4)) * 32 + c % 2 * 16
+                    : r / 4 * 128 + (r % 4 ^ (r / 4 % 2)) * 32 + c * 16;
+}
+template <int D>
+__device__ __forceinline__ uint32_t kv4_v_offset(int r, int c) {
+    return D == 128 ? r / 2 * 128 + r % 2 * 64 + (c ^ (r / 2 % 4)) * 16
+                    : r / 4 * 128 + r % 4 * 32 + (c ^ (r / 4 % 2)) * 16;
 }
 
 template <int D, int NT, int MT, int STAGES, int NW>
 struct Kv4Smem {
-    static constexpr int kStepBytes = 16 * MT * (D / 2);                // K (or V) of one step
+    static constexpr int kStepBytes = MT * kv4_block_bytes<D>();        // K (or V) of one step
     static constexpr int kWarpBytes = 2 * STAGES * kStepBytes;          // a warp's ring
     static constexpr size_t kRingBytes = size_t(NW) * kWarpBytes;
     static constexpr int kXFloats = (D / 16) * 4 + 4;
@@ -64,61 +76,105 @@ struct Kv4Smem {
     static constexpr size_t kMetaOffset = kFlagOffset + 16 * sizeof(int);
     static constexpr size_t kMetaBytes = (2 * kPersistMaxBatch + 1 + 16) * sizeof(int);
     static constexpr size_t kBytes = 1024 + kMetaOffset + kMetaBytes;   // the frame aligns to 1024
-    static_assert(kStepBytes % 128 == 0 && kScaleOffset % 16 == 0, "alignment");
+    static_assert(kStepBytes % 16 == 0 && kScaleOffset % 16 == 0, "alignment");
     // cached_merge reuses the exchange area: weights [threads] + 2 x heads
     static_assert(kXBytes >= (NW * 32 + 2 * NT * 8) * sizeof(float), "merge area");
 };
 
 // q of one item as the B operand, in the order in which masks bring K's codes:
 // of each word of eight dims 0, 4 and 2, 6 (low halves), 1, 5 and 3, 7 (high
-// ones).  sum: of each group's elements of the heads 2t, 2t + 1, times 2^-24.
+// ones).  Each head is first scaled by a power of two to 2^10 .. 2^11 at its
+// largest element; the low halves' elements then take 16 times as much, so that
+// both halves' products sum up in one accumulator without leaving fp16's range
+// (what that takes off is below 2^-35 of the largest element).  For the heads
+// 2t, 2t + 1: sum of each group's elements, in the same units as the products,
+// and unit, which takes a score from these to base 2.
 template <int D, int NT>
 struct Kv4Query {
     static constexpr int NG = D / kKv4Group;
     uint32_t b[NG][2][2][NT][2];                // group, word, low / high, tile of heads
-    float sum[NG][NT][2];
+    float sum[NG][NT][2], unit[NT][2];
 
-    __device__ __forceinline__ void load(const __half* q, int gcount, int lane) {
+    __device__ __forceinline__ void load(const __half* q, int gcount, float sl2, int lane) {
         const int g = lane >> 2, t = lane & 3;
         constexpr uint32_t kOnes = 0x3c003c00u;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int hj = nt * 8 + g;
             const __half* row = q + (size_t)hj * D + 16 * t;
+            uint4 v[NG][2];
+            __half2 top = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
 #pragma unroll
-            for (int x = 0; x < NG; ++x) {
-                float s[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int x = 0; x < NG; ++x)
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (hj < gcount) v = *reinterpret_cast<const uint4*>(row + x * kKv4Group + w * 8);
-                    b[x][w][0][nt][0] = __byte_perm(v.x, v.z, 0x5410);
-                    b[x][w][0][nt][1] = __byte_perm(v.y, v.w, 0x5410);
-                    b[x][w][1][nt][0] = __byte_perm(v.x, v.z, 0x7632);
-                    b[x][w][1][nt][1] = __byte_perm(v.y, v.w, 0x7632);
+                    v[x][w] = make_uint4(0, 0, 0, 0);
+                    if (hj < gcount) v[x][w] = *reinterpret_cast<const uint4*>(row + x * kKv4Group + w * 8);
+                    const uint32_t e[4] = {v[x][w].x, v[x][w].y, v[x][w].z, v[x][w].w};
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        mma_16816(s, kOnes, kOnes, kOnes, kOnes, b[x][w][e][nt][0], b[x][w][e][nt][1]);
+                    for (int i = 0; i < 4; ++i)
+                        top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(&e[i])));
                 }
-                sum[x][nt][0] = s[0] * 0x1p-24f;
-                sum[x][nt][1] = s[1] * 0x1p-24f;
+            const float2 two = __half22float2(top);
+            float big = fmaxf(two.x, two.y);
+            if (!(two.x < INFINITY && two.y < INFINITY)) big = 1.f;     // stays NaN or infinite
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            // 2^up: big's exponent e (-24 .. 15) becomes 10
+            const int up = big > 0.f ? 10 - (int(__float_as_uint(big) >> 23) - 127) : 0;
+            const float f = __int_as_float((127 + up) << 23);
+#pragma unroll
+            for (int x = 0; x < NG; ++x)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    uint32_t e[4] = {v[x][w].x, v[x][w].y, v[x][w].z, v[x][w].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&e[i]));
+                        e[i] = pack_half2(z.x * (f * 16.f), z.y * f);   // an even and an odd dim
+                    }
+                    b[x][w][0][nt][0] = __byte_perm(e[0], e[2], 0x5410);
+                    b[x][w][0][nt][1] = __byte_perm(e[1], e[3], 0x5410);
+                    b[x][w][1][nt][0] = __byte_perm(e[0], e[2], 0x7632);
+                    b[x][w][1][nt][1] = __byte_perm(e[1], e[3], 0x7632);
+                }
+#pragma unroll
+            for (int x = 0; x < NG; ++x) {
+                float s[4], s16[4];
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    auto add = [&](float (&acc)[4], int e) {
+                        if (w == 0) mma_16816_first(acc, kOnes, kOnes, kOnes, kOnes, b[x][w][e][nt][0], b[x][w][e][nt][1]);
+                        else mma_16816(acc, kOnes, kOnes, kOnes, kOnes, b[x][w][e][nt][0], b[x][w][e][nt][1]);
+                    };
+                    add(s16, 0);
+                    add(s, 1);
+                }
+                sum[x][nt][0] = fmaf(s[0], 16.f, s16[0]) * 0x1p-24f;
+                sum[x][nt][1] = fmaf(s[1], 16.f, s16[1]) * 0x1p-24f;
             }
+            // products: 2^-24 (codes) * 16 * 2^up
+            const float back = sl2 * 0x1p20f * __int_as_float((127 - up) << 23);
+            unit[nt][0] = __shfl_sync(0xffffffffu, back, 8 * t);
+            unit[nt][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
         }
     }
 };
 
-// Running state of a warp over an item, per head column.  r[g] is the reference
-// of group g's weights, in base 2 and a whole number; f = 2^(r[0] - r[g]).
-// o, z: products with V's codes and with 8, in units of 2^-24; mid: this lane's
-// rows' part of sum p mid, l that of the row sum, both on r[0].
+// Running state of a warp over an item, per head column.  r is the reference of
+// the first group's weights, in base 2 and a whole number, f[x] 2^(r - that of
+// group x).  o: products with V's codes, in units of 2^-24 (even dims) and 2^-28
+// (odd ones); z: 8 times the weights' sum, in units of 2^-24; mid: this lane's
+// rows' part of sum p mid, l that of the row sum, both on r.
 template <int D, int NT>
 struct Kv4State {
     static constexpr int NG = D / kKv4Group;
     float o[D / 16][NT][4], z[NG][NT][4];
     float mid[NG][NT][2], l[NT][2];
-    float r[NG][NT][2], f[NG][NT][2];
+    float r[NT][2], f[NG][NT][2];               // f[0] is 1
     float m[NT][2];
     bool fresh;                                 // nothing summed yet: no references
+    int blocks;                                 // since z was last taken off
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -128,21 +184,46 @@ struct Kv4State {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[dm][nt][c] = 0.f;
 #pragma unroll
-            for (int x = 0; x < NG; ++x) {
+            for (int x = 0; x < NG; ++x)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) z[x][nt][c] = 0.f;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    mid[x][nt][j] = r[x][nt][j] = 0.f;
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int x = 0; x < NG; ++x) {
+                    mid[x][nt][j] = 0.f;
                     f[x][nt][j] = 1.f;
                 }
+                r[nt][j] = l[nt][j] = 0.f;
             }
-            l[nt][0] = l[nt][1] = 0.f;
         }
         fresh = true;
+        blocks = 0;
     }
-    // Sums over the warp's rows, o whole and on r[0]: the (m, l, o) of the merges.
+    // Takes 8 times the weights' sum off the products with the codes.  Left to
+    // the end, what the products' sums lose by rounding would grow with the
+    // length while the outputs shrink: 64 sequences of 8192 to 32768 tokens were
+    // off by 4.8e-4 of the outputs' 2-norm instead of 2.4e-4.
+    __device__ __forceinline__ void centre() {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < NG; ++x) {
+#pragma unroll
+                for (int dm = 4 * x; dm < 4 * x + 4; ++dm)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        o[dm][nt][j] -= z[x][nt][j];
+                        o[dm][nt][j + 2] = fmaf(-16.f, z[x][nt][j], o[dm][nt][j + 2]);
+                    }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) z[x][nt][c] = 0.f;
+            }
+        blocks = 0;
+    }
+    // Sums over the warp's rows, o whole and on r: the (m, l, o) of the merges.
     __device__ __forceinline__ void finish() {
+        centre();
         auto rows = [](float x) {
             x += __shfl_xor_sync(0xffffffffu, x, 4);
             x += __shfl_xor_sync(0xffffffffu, x, 8);
@@ -153,77 +234,74 @@ struct Kv4State {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 l[nt][j] = rows(l[nt][j]);
-                m[nt][j] = fresh ? -INFINITY : r[0][nt][j];
+                m[nt][j] = fresh ? -INFINITY : r[nt][j];
 #pragma unroll
                 for (int x = 0; x < NG; ++x) {
                     const float c = rows(mid[x][nt][j]);
-                    const float u = 0x1p24f * fast_exp2(r[x][nt][j] - r[0][nt][j]);
+                    const float u = x ? 0x1p24f / f[x][nt][j] : 0x1p24f;
 #pragma unroll
                     for (int dm = 4 * x; dm < 4 * x + 4; ++dm) {
-                        o[dm][nt][j] = fmaf(o[dm][nt][j] - z[x][nt][j], u, c);
-                        o[dm][nt][j + 2] = fmaf(fmaf(o[dm][nt][j + 2], 0.0625f, -z[x][nt][j]), u, c);
+                        o[dm][nt][j] = fmaf(o[dm][nt][j], u, c);
+                        o[dm][nt][j + 2] = fmaf(o[dm][nt][j + 2], 0.0625f * u, c);
                     }
                 }
             }
     }
 };
 
-// One step: 16 * MT rows of K at kst and V at vst, of which the first `valid`
-// (>= 1) are positions; sc: their scales.
-template <int D, int NT, int MT, bool REST>
-__device__ __forceinline__ void consume_kv4(uint32_t kst, uint32_t vst, uint32_t sc, int valid,
-                                            const Kv4Query<D, NT>& q, Kv4State<D, NT>& st,
-                                            float sl2, int lane) {
-    constexpr int NG = D / kKv4Group;
-    const int g = lane >> 2, t = lane & 3;
-    const int rg = kv4_pos_of(g);               // rows of the A fragments: rg, rg + 8
-    const bool tail = valid < 16 * MT;          // uniform over the warp
-    const float unit = sl2 * 0x1p24f;
+// Where a lane's parts of a block lie: K's groups of an even row and of the odd
+// one after it, a 16-byte chunk of a row in each group of V, the two rows' scales.
+template <int D>
+struct Kv4Lane {
+    static constexpr int NG = D / kKv4Group;
+    uint32_t k[2][NG], v[NG], scales;
 
-    // ---- scores (times 2^-24), and V's scales and middles of the lane's rows
-    float s[MT][NT][4];
-    float va[MT][2][NG], vm[MT][2][NG];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        float ka[2][NG], kb[2][NG];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = mt * 16 + rg + 8 * i;
-            uint32_t w[2 * NG];                 // K's groups, V's groups
-            if constexpr (NG == 2) {
-                const uint4 x = lds128(sc + row * 16);
-                w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-            } else {
-                const uint2 x = lds64(sc + row * 8);
-                w[0] = x.x; w[1] = x.y;
-            }
-            // What rows past the end hold is anything, a NaN included.
-            if (tail && row >= valid) {
-#pragma unroll
-                for (int x = 0; x < NG; ++x) w[NG + x] = 0u;
-            }
-#pragma unroll
-            for (int x = 0; x < NG; ++x) {
-                const float2 kp = __half22float2(*reinterpret_cast<const __half2*>(&w[x]));
-                const float2 vp = __half22float2(*reinterpret_cast<const __half2*>(&w[NG + x]));
-                ka[i][x] = kp.x;
-                kb[i][x] = kp.y;
-                va[mt][i][x] = vp.x;
-                vm[mt][i][x] = fmaf(8.f, vp.x, vp.y);
-            }
-        }
-        float d[NG][2][NT][4];                  // q . n of the low halves, 16 q . n of the high ones
+    __device__ __forceinline__ Kv4Lane(uint32_t kst, uint32_t vst, uint32_t sc, int lane) {
+        const int r = (lane >> 2) * 2;
 #pragma unroll
         for (int x = 0; x < NG; ++x) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int i = 0; i < 2; ++i) k[i][x] = kst + kv4_k_offset<D>(r + i, 2 * x) + lane % 4 * 8;
+            v[x] = vst + kv4_v_offset<D>(lane % 16, 2 * x + lane / 16);
+        }
+        scales = sc + r * (8 * NG);
+    }
+};
+
+// A block of 16 rows on its way through a warp: scores, weights, then the products
+// with V.
+template <int D, int NT, bool REST>
+struct Kv4Block {
+    static constexpr int NG = D / kKv4Group;
+    float s[NT][4];                             // scores, in units of q.unit
+    float va[2][NG], vm[2][NG];                 // V's scales and middles of the lane's rows
+    uint32_t w[NG][NT][2], rest[NG][NT][2];     // weights, and what their rounding took off
+
+    static __device__ __forceinline__ float2 wide(uint32_t h) {
+        return __half22float2(*reinterpret_cast<const __half2*>(&h));
+    }
+
+    // TAIL: only the first `valid` (>= 1) rows are positions.
+    template <bool TAIL>
+    __device__ __forceinline__ void score(const Kv4Lane<D>& at, int block, int valid,
+                                          const Kv4Query<D, NT>& q, int lane) {
+        uint32_t pair[2][2 * NG];               // of rows 2 g, 2 g + 1: K's groups, V's groups
+        {
+            const uint4 x = lds128(at.scales + block * (16 * 8 * NG));
+            if constexpr (NG == 2) {
+                const uint4 y = lds128(at.scales + block * (16 * 8 * NG) + 16);
+                pair[0][0] = x.x; pair[0][1] = x.y; pair[0][2] = x.z; pair[0][3] = x.w;
+                pair[1][0] = y.x; pair[1][1] = y.y; pair[1][2] = y.z; pair[1][3] = y.w;
+            } else {
+                pair[0][0] = x.x; pair[0][1] = x.y;
+                pair[1][0] = x.z; pair[1][1] = x.w;
+            }
+        }
+        float d[NG][NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) d[x][e][nt][c] = 0.f;
-            const int at = x * (kKv4Group / 2) + 8 * t;
-            const uint2 lo = lds64(kst + kv4_offset<D>(mt * 16 + rg, at));
-            const uint2 hi = lds64(kst + kv4_offset<D>(mt * 16 + rg + 8, at));
+        for (int x = 0; x < NG; ++x) {
+            const uint2 lo = lds64(at.k[0][x] + block * kv4_block_bytes<D>());
+            const uint2 hi = lds64(at.k[1][x] + block * kv4_block_bytes<D>());
             const uint32_t xs[2] = {lo.x, lo.y}, ys[2] = {hi.x, hi.y};
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
@@ -232,243 +310,271 @@ __device__ __forceinline__ void consume_kv4(uint32_t kst, uint32_t vst, uint32_t
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t mask = e ? kHighHalves : kLowHalves;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        mma_16816(d[x][e][nt], xs[w] & mask, ys[w] & mask, x8 & mask, y8 & mask,
-                                  q.b[x][w][e][nt][0], q.b[x][w][e][nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (w + e == 0)
+                            mma_16816_first(d[x][nt], xs[w] & mask, ys[w] & mask, x8 & mask, y8 & mask,
+                                            q.b[x][w][e][nt][0], q.b[x][w][e][nt][1]);
+                        else
+                            mma_16816(d[x][nt], xs[w] & mask, ys[w] & mask, x8 & mask, y8 & mask,
+                                      q.b[x][w][e][nt][0], q.b[x][w][e][nt][1]);
+                    }
                 }
             }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int i = 0; i < 2; ++i) {
+            float2 k[NG];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int i = c >> 1, j = c & 1;
-                float sum = 0.f;
-#pragma unroll
-                for (int x = 0; x < NG; ++x) {
-                    sum = fmaf(kb[i][x], q.sum[x][nt][j], sum);
-                    sum = fmaf(ka[i][x], fmaf(d[x][1][nt][c], 0.0625f, d[x][0][nt][c]), sum);
-                }
-                s[mt][nt][c] = sum;
-                if (tail && mt * 16 + rg + 8 * i >= valid) s[mt][nt][c] = -INFINITY;
+            for (int x = 0; x < NG; ++x) {
+                k[x] = wide(pair[i][x]);
+                const float2 a = wide(pair[i][NG + x]);
+                va[i][x] = a.x;
+                vm[i][x] = fmaf(8.f, a.x, a.y);
             }
-    }
-
-    // ---- probabilities and weights on the references as they are
-    float p[MT][NT][4], w[MT][NG][NT][4];
-    bool over = false;
-    auto weigh = [&]() {
-        float top_p = 0.f, top_w = 0.f;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const float pc = fast_exp2(fmaf(s[mt][nt][c], unit, -st.r[0][nt][c & 1]));
-                    p[mt][nt][c] = pc;
-                    top_p = fmaxf(top_p, pc);
+                for (int j = 0; j < 2; ++j) {
+                    float sum = k[0].y * q.sum[0][nt][j];
 #pragma unroll
                     for (int x = 0; x < NG; ++x) {
-                        const float wc = (x ? pc * st.f[x][nt][c & 1] : pc) * va[mt][c >> 1][x];
-                        w[mt][x][nt][c] = wc;
-                        top_w = fmaxf(top_w, wc);
+                        if (x) sum = fmaf(k[x].y, q.sum[x][nt][j], sum);
+                        sum = fmaf(k[x].x, d[x][nt][2 * i + j], sum);
                     }
+                    s[nt][2 * i + j] = sum;
                 }
-        over = top_w > 0x1p15f || top_p > 0x1p39f;
-    };
-    weigh();
-    if (__any_sync(0xffffffffu, over || st.fresh)) {
-        // Move the references that a weight has outgrown to the weights' maxima
-        // and rescale what is summed so far.  A column and group moves for its
-        // own weights only: no head's bits depend on another's.
+            // What rows past the end hold is anything, a NaN included.
+            if (TAIL && (lane >> 2) * 2 + i >= valid) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+                for (int x = 0; x < NG; ++x) va[i][x] = vm[i][x] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                for (int x = 0; x < NG; ++x) {
-                    const float r0 = st.r[x][nt][j];
-                    float top = -INFINITY;      // log2 of the largest weight on r0
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            top = fmaxf(top, fmaf(s[mt][nt][2 * i + j], unit, -r0) +
-                                                 fmaxf(fast_log2(va[mt][i][x]), kKv4Least));
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1)
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    const bool move = st.fresh ? top > -INFINITY : top > kKv4Top;
-                    const float by = move ? rintf(top - kKv4Shift) : 0.f;
-                    st.r[x][nt][j] = r0 + by;
-                    // without a reference the sums are 0
-                    const float u = st.fresh || !move ? 1.f : fast_exp2(-by);
-#pragma unroll
-                    for (int dm = 4 * x; dm < 4 * x + 4; ++dm) {
-                        st.o[dm][nt][j] *= u;
-                        st.o[dm][nt][j + 2] *= u;
-                    }
-                    st.z[x][nt][j] *= u;
-                    if (x == 0) {
-                        st.l[nt][j] *= u;
-#pragma unroll
-                        for (int y = 0; y < NG; ++y) st.mid[y][nt][j] *= u;
-                    }
-                    st.f[x][nt][j] = fast_exp2(st.r[0][nt][j] - st.r[x][nt][j]);
-                }
+                for (int nt = 0; nt < NT; ++nt) s[nt][2 * i] = s[nt][2 * i + 1] = -INFINITY;
             }
-        st.fresh = false;
-        weigh();
+        }
     }
 
-    // ---- row sums and middles (unrounded p); W^T = P^T a' as fp16 in the B
-    // layout (k = position, n = head)
-    uint32_t wb[MT][NG][NT][2], wr[MT][NG][NT][2];
+    // Probabilities, their sums, and the weights P^T a' as fp16.  Where the weights
+    // of a column's rows here sum up to 2^15 or more (in fp32, on a pipe with room;
+    // with p as weights of the least scale among them), the column's references move.
+    __device__ __forceinline__ void weigh(const Kv4Query<D, NT>& q, Kv4State<D, NT>& st, int lane) {
+        float p[NT][4], ps[NT][2], all[NT][2];
+        bool over = false;
+        auto form = [&]() {
+            over = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+                for (int c = 0; c < 4; ++c)
+                    p[nt][c] = fast_exp2(fmaf(s[nt][c], q.unit[nt][c & 1], -st.r[nt][c & 1]));
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                st.l[nt][c & 1] += p[mt][nt][c];
+                for (int j = 0; j < 2; ++j) {
+                    ps[nt][j] = p[nt][j] + p[nt][2 + j];
+                    all[nt][j] = ps[nt][j] * 0x1p-24f;
+                }
 #pragma unroll
                 for (int x = 0; x < NG; ++x)
-                    st.mid[x][nt][c & 1] = fmaf(p[mt][nt][c], vm[mt][c >> 1][x], st.mid[x][nt][c & 1]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float w0 = p[nt][2 * i], w1 = p[nt][2 * i + 1];
+                        if (x) {
+                            w0 *= st.f[x][nt][0];
+                            w1 *= st.f[x][nt][1];
+                        }
+                        w0 *= va[i][x];
+                        w1 *= va[i][x];
+                        all[nt][0] += w0;
+                        all[nt][1] += w1;
+                        const uint32_t h = pack_half2(w0, w1);
+                        w[x][nt][i] = h;
+                        if constexpr (REST) {
+                            const float2 r = wide(h);
+                            rest[x][nt][i] = pack_half2(w0 - r.x, w1 - r.y);
+                        }
+                    }
+                over |= fmaxf(all[nt][0], all[nt][1]) > kKv4Most;
             }
+        };
+        form();
+        if (__any_sync(0xffffffffu, over || st.fresh)) {
+            // Rescale what is summed so far to the weights' new references.  A column
+            // moves for its own weights only: no head's bits depend on another's.
 #pragma unroll
-            for (int x = 0; x < NG; ++x)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float w0 = w[mt][x][nt][2 * e], w1 = w[mt][x][nt][2 * e + 1];
-                    const uint32_t h = pack_half2(w0, w1);
-                    wb[mt][x][nt][e] = movmatrix_trans(h);
-                    if constexpr (REST) {
-                        const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                        wr[mt][x][nt][e] = movmatrix_trans(pack_half2(w0 - r.x, w1 - r.y));
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t column = 0x11111111u << (lane & 3);
+                    const bool move = st.fresh || (__ballot_sync(0xffffffffu, all[nt][j] > kKv4Most) & column);
+                    const float r0 = st.r[nt][j];
+                    float by0 = 0.f;
+#pragma unroll
+                    for (int x = 0; x < NG; ++x) {
+                        float top = -INFINITY;  // log2 of the largest weight as it is
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            top = fmaxf(top, fmaf(s[nt][2 * i + j], q.unit[nt][j], -r0) +
+                                                 fmaxf(fast_log2(va[i][x]), kKv4Least));
+                        if (x) top += fast_log2(st.f[x][nt][j]);
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1)
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        // up only, but from no reference to any
+                        float by = rintf(top - kKv4Shift);
+                        if (!move || !(by > (st.fresh ? -INFINITY : 0.f))) by = 0.f;
+                        // without a reference the sums are 0
+                        const float u = st.fresh ? 1.f : fast_exp2(-by);
+#pragma unroll
+                        for (int dm = 4 * x; dm < 4 * x + 4; ++dm) {
+                            st.o[dm][nt][j] *= u;
+                            st.o[dm][nt][j + 2] *= u;
+                        }
+                        st.z[x][nt][j] *= u;
+                        if (x == 0) {
+                            by0 = by;
+                            st.r[nt][j] = r0 + by;
+                            st.l[nt][j] *= u;
+#pragma unroll
+                            for (int y = 0; y < NG; ++y) st.mid[y][nt][j] *= u;
+                        } else {
+                            st.f[x][nt][j] *= fast_exp2(by0 - by);
+                        }
                     }
                 }
+            st.fresh = false;
+            form();
         }
-
-    // ---- O^T += V^T W^T, and z
-    const int p0 = kv4_pos_of(2 * t), p1 = kv4_pos_of(2 * t + 1);
-    constexpr uint32_t kEight = 0x00080008u;
+        // row sums and middles, of the unrounded p
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) st.l[nt][j] += ps[nt][j];
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int x = 0; x < NG; ++x)
+                    st.mid[x][nt][c & 1] = fmaf(p[nt][c], vm[c >> 1][x], st.mid[x][nt][c & 1]);
+        }
+    }
+
+    // O^T += V^T W^T and z, the weights in the B layout (k = position, n = head).
+    __device__ __forceinline__ void apply(const Kv4Lane<D>& at, int block, Kv4State<D, NT>& st) const {
+        constexpr uint32_t kEight = 0x00080008u;
 #pragma unroll
         for (int x = 0; x < NG; ++x) {
-            const int at = x * (kKv4Group / 2) + 4 * g;
-            uint32_t v[4];                      // rows p0, p1, p0 + 8, p1 + 8
+            uint32_t v[4], wb[NT][2], wr[NT][2];
+            ldsm_b8_trans(v, at.v[x] + block * kv4_block_bytes<D>());
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                v[i] = lds32(vst + kv4_offset<D>(mt * 16 + (i & 1 ? p1 : p0) + (i >> 1) * 8, at));
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    wb[nt][i] = movmatrix_trans(w[x][nt][i]);
+                    if constexpr (REST) wr[nt][i] = movmatrix_trans(rest[x][nt][i]);
+                }
             auto product = [&](float (&acc)[NT][4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-                    mma_16816(acc[nt], a0, a1, a2, a3, wb[mt][x][nt][0], wb[mt][x][nt][1]);
+                for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt], a0, a1, a2, a3, wb[nt][0], wb[nt][1]);
                 if constexpr (REST) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        mma_16816(acc[nt], a0, a1, a2, a3, wr[mt][x][nt][0], wr[mt][x][nt][1]);
+                    for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt], a0, a1, a2, a3, wr[nt][0], wr[nt][1]);
                 }
             };
             product(st.z[x], kEight, kEight, kEight, kEight);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {       // dims 4e .. 4e + 3 of the lane's eight
-                const uint32_t lo = __byte_perm(v[0], v[1], e ? 0x7632 : 0x5410);
-                const uint32_t hi = __byte_perm(v[2], v[3], e ? 0x7632 : 0x5410);
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const uint32_t l8 = y ? lo >> 8 : lo, h8 = y ? hi >> 8 : hi;
-                    product(st.o[4 * x + 2 * e + y], l8 & kLowHalves, l8 & kHighHalves,
-                            h8 & kLowHalves, h8 & kHighHalves);
-                }
+            for (int y = 0; y < 4; ++y) {       // dims 16 y + 2 g, + 1 of the group
+                const uint32_t v8 = v[y] >> 8;
+                product(st.o[4 * x + y], v[y] & kLowHalves, v[y] & kHighHalves, v8 & kLowHalves,
+                        v8 & kHighHalves);
             }
         }
-}
+    }
+};
 
-// Where a warp's copies are: the tile of its cursor and, looked up already,
-// the pages of the warp's MT blocks of it (-1 where there is no position,
-// num_pages for an id outside the pool).  The page index and the block within
-// the page go along with the cursor, without divisions.
+// Where a warp's copies are: the tile of its cursor and, looked up already, the
+// pages of the warp's MT blocks of it (-1: nothing to copy, zeros are filled in:
+// a block without positions or a page id outside the pool).  The page index, the
+// block within the page and the positions left go along with the cursor; what
+// depends on the sequence and head is formed where these change.
 template <int D, int MT, int NW>
 struct Kv4Loader {
-    static constexpr int CPR = D / 32;          // 16-byte chunks per row
-    static constexpr int RPC = 32 / CPR;        // rows per warp-wide copy
     static constexpr int kBlock = 16;
+    static constexpr int LPB = 32 / MT;         // lanes per block
+    static constexpr int CPR = D / 32;          // 16-byte chunks per row
+    static constexpr int RPC = LPB / CPR;       // rows of a block per warp-wide copy
     static constexpr int kRowScales = 8 * (D / kKv4Group);
+    static constexpr int kTile = kBlock * MT * NW;
+    static_assert(32 % MT == 0 && kRowScales <= LPB && LPB % CPR == 0 && RPC % 2 == 0, "lanes of a block");
     TileCursor cur;
-    int idx, sub;                               // page index and block within it, first block
-    int bpp, step_idx, step_sub, idx0, sub0;    // blocks per page; NW * MT blocks; tile 0
-    int page[MT];
-    long long lane_off;
+    int idx, sub, left;                         // the lane's block: page index, block within the page, positions from there on
+    int page;
+    int bpp, step_idx, step_sub;                // blocks per page; NW * MT blocks
+    const int* row;                             // the sequence's pages
+    uint32_t off, scale_off;                    // the lane's chunk in the kv head's part of page 0, in 16 bytes
+    uint32_t k_dst, v_dst, scale_dst;           // ... and in a step in shared memory
 
+    __device__ __forceinline__ void unit(const CachedDecodeParams<Kv4View>& p, const int* lens, int warp,
+                                         int lane) {
+        const int kvh = p.head_groups == 1 ? cur.j : cur.j / p.head_groups;
+        const int blk = (cur.i * NW + warp) * MT + lane / LPB;
+        idx = blk / bpp;
+        sub = blk - idx * bpp;
+        off = (uint32_t)(p.cache.row(0, kvh, lane % LPB / CPR) >> 4) + lane % CPR;
+        scale_off = kvh * p.cache.head_scales16 + lane % LPB;
+        row = p.block_table + (size_t)cur.b * p.bt_stride;
+        left = (cur.b < p.batch ? lens[cur.b] : 0) - blk * kBlock;
+    }
     __device__ __forceinline__ void init(const CachedDecodeParams<Kv4View>& p, const TileCursor& start,
                                          const int* lens, int warp, int lane) {
         cur = start;
         bpp = p.cache.page_size / kBlock;
         step_idx = NW * MT / bpp;
         step_sub = NW * MT - step_idx * bpp;
-        idx0 = warp * MT / bpp;
-        sub0 = warp * MT - idx0 * bpp;
-        const int blk = (cur.i * NW + warp) * MT;
-        idx = blk / bpp;
-        sub = blk - idx * bpp;
-        lane_off = (long long)(lane / CPR) * p.cache.row_stride + (lane % CPR) * 16;
+        const int c = lane % CPR, r = lane % LPB / CPR, block = lane / LPB * kv4_block_bytes<D>();
+        k_dst = block + kv4_k_offset<D>(r, c);
+        v_dst = block + kv4_v_offset<D>(r, c);
+        scale_dst = lane / LPB * (kBlock * kRowScales) + lane % LPB * 16;
+        unit(p, lens, warp, lane);
         look_up(p, lens, warp);
     }
-    __device__ __forceinline__ void look_up(const CachedDecodeParams<Kv4View>& p, const int* lens,
-                                            int warp) {
-        const int pos = (cur.i * NW + warp) * (kBlock * MT);
-        const int left = cur.b < p.batch ? lens[cur.b] - pos : 0;
-        const int* row = p.block_table + (size_t)cur.b * p.bt_stride;
-        int at = idx, s = sub;
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            page[m] = -1;
-            if (kBlock * m < left) page[m] = min((unsigned)row[at], (unsigned)p.cache.num_pages);
-            if (++s == bpp) { s = 0; ++at; }
+    __device__ __forceinline__ void look_up(const CachedDecodeParams<Kv4View>& p, const int*, int) {
+        page = -1;
+        if (left > 0) {
+            const int id = row[idx];
+            if ((unsigned)id < (unsigned)p.cache.num_pages) page = id;
         }
     }
     // Starts the copies of the step: 16 rows of K and of V and their scales of
-    // each block that holds positions; zeros for a page outside the pool.
+    // each block.
     __device__ __forceinline__ void copy(const CachedDecodeParams<Kv4View>& p, uint32_t kst, uint32_t vst,
-                                         uint32_t scale_at, int kvh, int lane, uint64_t policy) const {
-        const int r0 = lane / CPR, c = lane % CPR;
-        int s = sub;
+                                         uint32_t scale_at, int, int lane, uint64_t policy) const {
+        // 32-bit numbers of 16 bytes: the host checks that a cache has no more.
+        const uint32_t row_stride = p.cache.block16;
+        const uint32_t bytes = page >= 0 ? 16u : 0u;
+        const uint32_t pg = max(page, 0);
+        const size_t at = (size_t)(off + pg * p.cache.page16 + sub * row_stride) * 16;
+        const uint8_t* ks = p.cache.k + at;
+        const uint8_t* vs = p.cache.v + at;
+        auto rows = [&](auto stride) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            if (page[m] >= 0) {                 // uniform over the warp
-                const bool real = page[m] < p.cache.num_pages;
-                const int pg = real ? page[m] : 0;
-                const uint32_t bytes = real ? 16u : 0u;
-                const long long off = pg * p.cache.page_stride + kvh * p.cache.head_stride +
-                                      s * kBlock * p.cache.row_stride + lane_off;
-                const uint8_t* ks = p.cache.k + off;
-                const uint8_t* vs = p.cache.v + off;
-#pragma unroll
-                for (int i = 0; i < kBlock / RPC; ++i) {
-                    const uint32_t dst = kv4_offset<D>(m * kBlock + i * RPC + r0, c * 16);
-                    cp_async_16(kst + dst, ks, bytes, policy);
-                    cp_async_16(vst + dst, vs, bytes, policy);
-                    ks += RPC * p.cache.row_stride;
-                    vs += RPC * p.cache.row_stride;
-                }
-                if (lane < kRowScales)          // 16 rows of kRowScales bytes, 16 a lane
-                    cp_async_16(scale_at + m * (kBlock * kRowScales) + lane * 16,
-                                reinterpret_cast<const char*>(
-                                    p.cache.pairs<D>(pg, kvh, s * kBlock)) + lane * 16,
-                                bytes, policy);
+            for (int i = 0; i < kBlock / RPC; ++i) {
+                const int line = i * RPC / (256 / D), turn = line % (D == 128 ? 4 : 2);     // what i * RPC rows add
+                cp_async_16(kst + (k_dst ^ (turn * 32)) + line * 128, ks + (size_t)stride * (i * RPC), bytes, policy);
+                cp_async_16(vst + (v_dst ^ (turn * 16)) + line * 128, vs + (size_t)stride * (i * RPC), bytes, policy);
             }
-            if (++s == bpp) s = 0;
+        };
+        if (row_stride == D / 2) rows(std::integral_constant<uint32_t, D / 2>());
+        else rows(row_stride);
+        if (kRowScales == LPB || lane % LPB < kRowScales) {     // 16 rows of kRowScales bytes, 16 a lane
+            const uint32_t from = scale_off + pg * p.cache.scales16 + sub * kRowScales;
+            cp_async_16(scale_at + scale_dst, reinterpret_cast<const uint8_t*>(p.cache.scales) + (size_t)from * 16,
+                        bytes, policy);
         }
     }
-    __device__ __forceinline__ void advance(const int* seq_start, int B, int upb) {
+    __device__ __forceinline__ void advance(const CachedDecodeParams<Kv4View>& p, const int* seq_start,
+                                            const int* lens, int B, int upb, int warp, int lane) {
         cur.advance(seq_start, B, upb, 1);
         if (cur.i == 0) {                       // next unit
-            idx = idx0;
-            sub = sub0;
+            unit(p, lens, warp, lane);
         } else {
+            left -= kTile;
             idx += step_idx;
             sub += step_sub;
             if (sub >= bpp) { sub -= bpp; ++idx; }
@@ -479,7 +585,7 @@ struct Kv4Loader {
 // Steps of MT blocks of 16 rows; CTAS per SM; REST as above.
 template <int D, int NT, int MT, int STAGES, int NW, int CTAS, bool REST>
 struct Kv4Format {
-    static constexpr int kD = D, kNT = NT, kMT = MT, kStages = STAGES, kNW = NW, kCtas = CTAS;
+    static constexpr int kD = D, kNT = NT, kMT = MT, kStages = STAGES, kNW = NW, kCtas = CTAS, kRun = 1;
     using Params = CachedDecodeParams<Kv4View>;
     using Smem = Kv4Smem<D, NT, MT, STAGES, NW>;
     using Loader = Kv4Loader<D, MT, NW>;
@@ -487,12 +593,34 @@ struct Kv4Format {
     using State = Kv4State<D, NT>;
 
     static __device__ __forceinline__ int dim(int dm, int g) {
-        return (dm >> 2) * kKv4Group + 8 * g + 2 * (dm & 3);
+        return (dm >> 2) * kKv4Group + 16 * (dm & 3) + 2 * g;
     }
     static __device__ __forceinline__ void consume(uint32_t kst, uint32_t vst, const unsigned char* sc,
-                                                   int valid, const Query& q, State& st, float sl2,
+                                                   int valid, const Query& q, State& st, float,
                                                    int lane) {
-        consume_kv4<D, NT, MT, REST>(kst, vst, smem_u32(sc), valid, q, st, sl2, lane);
+        const Kv4Lane<D> at(kst, vst, smem_u32(sc), lane);
+        if ((st.blocks += MT) > kKv4Centre) st.centre();        // uniform over the warp
+        if (valid >= 16 * MT) {
+            // The next block's scores beside the products of the one before it.
+            Kv4Block<D, NT, REST> b[2];
+            b[0].template score<false>(at, 0, 16, q, lane);
+            b[0].weigh(q, st, lane);
+#pragma unroll
+            for (int i = 1; i < MT; ++i) {
+                b[i % 2].template score<false>(at, i, 16, q, lane);
+                b[(i - 1) % 2].apply(at, i - 1, st);
+                b[i % 2].weigh(q, st, lane);
+            }
+            b[(MT - 1) % 2].apply(at, MT - 1, st);
+        } else {
+#pragma unroll 1
+            for (int i = 0; i * 16 < valid; ++i) {
+                Kv4Block<D, NT, REST> b;
+                b.template score<true>(at, i, valid - i * 16, q, lane);
+                b.weigh(q, st, lane);
+                b.apply(at, i, st);
+            }
+        }
     }
 };
 

@@ -141,7 +141,7 @@ template <int D, int NT>
 struct Kv8Query {
     uint32_t b[D / 16][NT][2];
 
-    __device__ __forceinline__ void load(const __half* q, int gcount, int lane) {
+    __device__ __forceinline__ void load(const __half* q, int gcount, float, int lane) {
         const int g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -428,7 +428,8 @@ struct Kv8Loader {
             if (++s == bpp) s = 0;
         }
     }
-    __device__ __forceinline__ void advance(const int* seq_start, int B, int upb) {
+    __device__ __forceinline__ void advance(const CachedDecodeParams<Kv8View>&, const int* seq_start,
+                                            const int*, int B, int upb, int, int) {
         cur.advance(seq_start, B, upb, 1);
         if (cur.i == 0) {                       // next unit
             idx = idx0;
@@ -444,7 +445,7 @@ struct Kv8Loader {
 // Steps of MT blocks of 16 rows; CTAS per SM; REST as in consume_kv8.
 template <int D, int NT, int MT, int STAGES, int NW, int CTAS, bool REST, class Code>
 struct Kv8Format {
-    static constexpr int kD = D, kNT = NT, kMT = MT, kStages = STAGES, kNW = NW, kCtas = CTAS;
+    static constexpr int kD = D, kNT = NT, kMT = MT, kStages = STAGES, kNW = NW, kCtas = CTAS, kRun = 4;
     using Params = CachedDecodeParams<Kv8View>;
     using Smem = Kv8Smem<D, NT, MT, STAGES, NW>;
     using Loader = Kv8Loader<D, MT, NW>;
