@@ -3,15 +3,17 @@
 // Mathematics, per (sequence, query head h of kv head j), positions t < len,
 // groups g of 64 dims with codes n, K's (a, b) and V's (a', b') as scale, bias:
 //   s_t = sum_g a_tg (q_g . n_tg) + b_tg (q_g . 1),  in units of 1 / sqrt(D)
-//   p_t = 2^(s_t log2 e - r),  l = sum_t p_t,  mid_tg = b'_tg + 8 a'_tg
-//   o_g = sum_t (p_t a'_tg) (n'_tg - 8) + sum_t p_t mid_tg,  out = o / l
+//   p_t = 2^(s_t log2 e - r),  l = sum_t p_t,  mid_tg = b'_tg + 7.5 a'_tg
+//   o_g = sum_t (p_t a'_tg) (n'_tg - 7.5) + sum_t p_t mid_tg,  out = o / l
 // (zeros for an empty sequence).  Codes enter the products as they are: the
 // fp16 with bits n is n 2^-24 exactly, so a mask makes two operands of a word,
 // n of the low halves and 16 n of the high ones, and the factors are taken off
-// the sums.  8 times the sum of the weights goes into a sum of its own by a
-// product with a constant operand (z), so that what rounding a weight to fp16
-// takes off counts by the distance from the group's middle, not from its
-// bottom (half the error).  Scores, l, o and all other sums are fp32.
+// the sums.  15 times the sum of a step's weights comes from a product with a
+// constant operand (z), and half of it is taken off o: what rounding a weight to
+// fp16 takes off then counts by the distance from the group's middle, not from its
+// bottom (half the error), and o stays small, so that its sums lose little (taken
+// off once at the end, outputs over 131072 positions were off by 3.2e-4 of their
+// 2-norm instead of 3.1e-4).  Scores, l, o and all other sums are fp32.
 //
 // A weight p a' enters the product with V as fp16 on a reference of its own
 // group's, 2^8 up, so that one as small as 2^-22 of the largest keeps all its
@@ -39,7 +41,6 @@ namespace fr {
 constexpr float kKv4Shift = 8.f;        // a weight at its reference counts 2^8 ...
 constexpr float kKv4Most = 0x1p15f;     // ... and the weights of a lane's rows may sum up to 2^15 before that moves
 constexpr float kKv4Least = -24.f;      // a smaller scale's reference is this scale's: p stays below 2^39
-constexpr int kKv4Centre = 16;          // blocks between two subtractions of z
 constexpr uint32_t kLowHalves = 0x000f000fu, kHighHalves = 0x00f000f0u;
 
 // A block (16 rows) in shared memory: lines of 128 bytes, of 2 rows (D = 128) or 4,
@@ -163,18 +164,17 @@ struct Kv4Query {
 
 // Running state of a warp over an item, per head column.  r is the reference of
 // the first group's weights, in base 2 and a whole number, f[x] 2^(r - that of
-// group x).  o: products with V's codes, in units of 2^-24 (even dims) and 2^-28
-// (odd ones); z: 8 times the weights' sum, in units of 2^-24; mid: this lane's
-// rows' part of sum p mid, l that of the row sum, both on r.
+// group x).  o: products with V's codes from 7.5 on, in units of 2^-24 (even dims)
+// and 2^-28 (odd ones); mid: this lane's rows' part of sum p mid, l that of the row
+// sum, both on r.
 template <int D, int NT>
 struct Kv4State {
     static constexpr int NG = D / kKv4Group;
-    float o[D / 16][NT][4], z[NG][NT][4];
+    float o[D / 16][NT][4];
     float mid[NG][NT][2], l[NT][2];
     float r[NT][2], f[NG][NT][2];               // f[0] is 1
     float m[NT][2];
     bool fresh;                                 // nothing summed yet: no references
-    int blocks;                                 // since z was last taken off
 
     __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -183,10 +183,6 @@ struct Kv4State {
             for (int dm = 0; dm < D / 16; ++dm)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[dm][nt][c] = 0.f;
-#pragma unroll
-            for (int x = 0; x < NG; ++x)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) z[x][nt][c] = 0.f;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
 #pragma unroll
@@ -198,32 +194,24 @@ struct Kv4State {
             }
         }
         fresh = true;
-        blocks = 0;
     }
-    // Takes 8 times the weights' sum off the products with the codes.  Left to
-    // the end, what the products' sums lose by rounding would grow with the
-    // length while the outputs shrink: 64 sequences of 8192 to 32768 tokens were
-    // off by 4.8e-4 of the outputs' 2-norm instead of 2.4e-4.
-    __device__ __forceinline__ void centre() {
+    // Takes 7.5 times the weights' sum off the products with the codes; z is 15
+    // times that sum, in units of 2^-24.
+    __device__ __forceinline__ void centre(const float (&z)[NG][NT][4]) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int x = 0; x < NG; ++x)
 #pragma unroll
-            for (int x = 0; x < NG; ++x) {
+            for (int dm = 4 * x; dm < 4 * x + 4; ++dm)
 #pragma unroll
-                for (int dm = 4 * x; dm < 4 * x + 4; ++dm)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        o[dm][nt][j] -= z[x][nt][j];
-                        o[dm][nt][j + 2] = fmaf(-16.f, z[x][nt][j], o[dm][nt][j + 2]);
+                        o[dm][nt][j] = fmaf(-0.5f, z[x][nt][j], o[dm][nt][j]);
+                        o[dm][nt][j + 2] = fmaf(-8.f, z[x][nt][j], o[dm][nt][j + 2]);
                     }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) z[x][nt][c] = 0.f;
-            }
-        blocks = 0;
     }
     // Sums over the warp's rows, o whole and on r: the (m, l, o) of the merges.
     __device__ __forceinline__ void finish() {
-        centre();
         auto rows = [](float x) {
             x += __shfl_xor_sync(0xffffffffu, x, 4);
             x += __shfl_xor_sync(0xffffffffu, x, 8);
@@ -329,7 +317,7 @@ struct Kv4Block {
                 k[x] = wide(pair[i][x]);
                 const float2 a = wide(pair[i][NG + x]);
                 va[i][x] = a.x;
-                vm[i][x] = fmaf(8.f, a.x, a.y);
+                vm[i][x] = fmaf(7.5f, a.x, a.y);
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -356,7 +344,10 @@ struct Kv4Block {
     // Probabilities, their sums, and the weights P^T a' as fp16.  Where the weights
     // of a column's rows here sum up to 2^15 or more (in fp32, on a pipe with room;
     // with p as weights of the least scale among them), the column's references move.
-    __device__ __forceinline__ void weigh(const Kv4Query<D, NT>& q, Kv4State<D, NT>& st, int lane) {
+    // ADDED: z holds what o does since it was last centred, and moves with it.
+    template <bool ADDED>
+    __device__ __forceinline__ void weigh(const Kv4Query<D, NT>& q, Kv4State<D, NT>& st,
+                                          float (&z)[NG][NT][4], int lane) {
         float p[NT][4], ps[NT][2], all[NT][2];
         bool over = false;
         auto form = [&]() {
@@ -427,7 +418,7 @@ struct Kv4Block {
                             st.o[dm][nt][j] *= u;
                             st.o[dm][nt][j + 2] *= u;
                         }
-                        st.z[x][nt][j] *= u;
+                        if constexpr (ADDED) z[x][nt][j] *= u;
                         if (x == 0) {
                             by0 = by;
                             st.r[nt][j] = r0 + by;
@@ -456,8 +447,11 @@ struct Kv4Block {
     }
 
     // O^T += V^T W^T and z, the weights in the B layout (k = position, n = head).
-    __device__ __forceinline__ void apply(const Kv4Lane<D>& at, int block, Kv4State<D, NT>& st) const {
-        constexpr uint32_t kEight = 0x00080008u;
+    // FIRST: z starts here.
+    template <bool FIRST>
+    __device__ __forceinline__ void apply(const Kv4Lane<D>& at, int block, Kv4State<D, NT>& st,
+                                          float (&z)[NG][NT][4]) const {
+        constexpr uint32_t kFifteen = 0x000f000fu;
 #pragma unroll
         for (int x = 0; x < NG; ++x) {
             uint32_t v[4], wb[NT][2], wr[NT][2];
@@ -477,7 +471,16 @@ struct Kv4Block {
                     for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt], a0, a1, a2, a3, wr[nt][0], wr[nt][1]);
                 }
             };
-            product(st.z[x], kEight, kEight, kEight, kEight);
+            if constexpr (FIRST) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma_16816_first(z[x][nt], kFifteen, kFifteen, kFifteen, kFifteen, wb[nt][0], wb[nt][1]);
+                    if constexpr (REST)
+                        mma_16816(z[x][nt], kFifteen, kFifteen, kFifteen, kFifteen, wr[nt][0], wr[nt][1]);
+                }
+            } else {
+                product(z[x], kFifteen, kFifteen, kFifteen, kFifteen);
+            }
 #pragma unroll
             for (int y = 0; y < 4; ++y) {       // dims 16 y + 2 g, + 1 of the group
                 const uint32_t v8 = v[y] >> 8;
@@ -599,26 +602,29 @@ struct Kv4Format {
                                                    int valid, const Query& q, State& st, float,
                                                    int lane) {
         const Kv4Lane<D> at(kst, vst, smem_u32(sc), lane);
-        if ((st.blocks += MT) > kKv4Centre) st.centre();        // uniform over the warp
+        float z[D / kKv4Group][NT][4];
         if (valid >= 16 * MT) {
             // The next block's scores beside the products of the one before it.
             Kv4Block<D, NT, REST> b[2];
             b[0].template score<false>(at, 0, 16, q, lane);
-            b[0].weigh(q, st, lane);
+            b[0].template weigh<false>(q, st, z, lane);
 #pragma unroll
             for (int i = 1; i < MT; ++i) {
                 b[i % 2].template score<false>(at, i, 16, q, lane);
-                b[(i - 1) % 2].apply(at, i - 1, st);
-                b[i % 2].weigh(q, st, lane);
+                if (i == 1) b[0].template apply<true>(at, 0, st, z);
+                else b[(i - 1) % 2].template apply<false>(at, i - 1, st, z);
+                b[i % 2].template weigh<true>(q, st, z, lane);
             }
-            b[(MT - 1) % 2].apply(at, MT - 1, st);
+            b[(MT - 1) % 2].template apply<MT == 1>(at, MT - 1, st, z);
+            st.centre(z);
         } else {
 #pragma unroll 1
             for (int i = 0; i * 16 < valid; ++i) {
                 Kv4Block<D, NT, REST> b;
                 b.template score<true>(at, i, valid - i * 16, q, lane);
-                b.weigh(q, st, lane);
-                b.apply(at, i, st);
+                b.template weigh<false>(q, st, z, lane);
+                b.template apply<true>(at, i, st, z);
+                st.centre(z);
             }
         }
     }
