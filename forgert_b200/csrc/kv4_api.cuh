@@ -287,9 +287,11 @@ int fr_kv4_gather(const fr_kv4_cache* cache, const long long* slots, void* k_out
         p.slots = slots;
         p.k_out = static_cast<__half*>(k_out);
         p.v_out = static_cast<__half*>(v_out);
-        p.pieces = (long long)num_slots * cache->num_kv_heads * (cache->head_dim / 16);
-        const long long grid = (p.pieces + 255) / 256;
-        if (grid >= (1LL << 31)) return FR_ERR_INVALID_ARG;
+        const long long rows = (long long)num_slots * cache->num_kv_heads;
+        if (rows >= 1LL << 31) return FR_ERR_INVALID_ARG;
+        p.rows = (uint32_t)rows;
+        const int per_cta = 256 / (cache->head_dim / 16);
+        const long long grid = (rows + per_cta - 1) / per_cta;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
         auto fn = cache->head_dim == 64 ? fr::kv4_gather_kernel<64> : fr::kv4_gather_kernel<128>;
         return launch_plain(fn, (unsigned)grid, 256, 0, s, static_cast<const fr::Kv4GatherParams>(p));

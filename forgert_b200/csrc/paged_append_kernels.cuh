@@ -18,6 +18,14 @@
 // 8l + 7, so that rows move in 16-byte accesses and a lane's codes are two whole
 // words.  No row depends on another: CTAs take rows of K, of V, and of q (kQRows
 // heads of a token to a lane group, which looks the angles up once).
+//
+// Bound: bytes and the latency of two rounds of loads (rows, slot and position;
+// then the angles).  4800 prompt tokens of 28 / 4 heads of 128 with biases, three
+// axes and 16-bit K and V written too, cold: 16-bit pages 19.1 us, 5.3 TB/s, 4 bits
+// 19.5.  It took 24.1 with the position looked up after the slot, rows through L1
+// (22.2: position early; 21.6: rows past L1) and four heads a lane group (20.4 with
+// two; 19.1 at nine CTAs per SM instead of eight, 24 at ten, where it spills; one
+// head, 22.5).  A decode step's 64 tokens take 2.2 and 2.6 in a graph.
 #pragma once
 #include "fr_ptx.cuh"
 #include "kv4_common.cuh"
@@ -26,8 +34,24 @@
 namespace fr {
 
 constexpr int kPagedThreads = 128;
+constexpr int kPagedCtas = 9;           // per SM: 56 registers
 constexpr int kPagedAxes = 4;
-constexpr int kQRows = 4;               // query rows that a lane group has under way
+constexpr int kQRows = 2;               // query rows that a lane group has under way
+
+// Page and row of a slot inside the pool (in 32 bits where they do: a 64-bit
+// division takes as long as coding a row).
+struct SlotPlace {
+    int page, row;
+    __device__ __forceinline__ SlotPlace(long long slot, int page_size) {
+        if (slot >> 32) {
+            page = int(slot / page_size);
+            row = int(slot - (long long)page * page_size);
+        } else {
+            page = (uint32_t)slot / (uint32_t)page_size;
+            row = (uint32_t)slot - (uint32_t)page * page_size;
+        }
+    }
+};
 
 struct PagedAppendParams {
     const __half* in[3];                // q, k, v
@@ -63,6 +87,15 @@ __device__ __forceinline__ void unpack8(uint4 w, float (&x)[8]) {
     }
 }
 
+// Sixteen bytes of a row, which is read once: past L1, which the angles and biases
+// of the next tokens stay in.
+__device__ __forceinline__ uint4 load_row(const __half* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
     return make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]),
                       pack_half2(x[6], x[7]));
@@ -74,22 +107,26 @@ __device__ __forceinline__ void store_row16(__half* row, int f0, const Row16& r)
     *reinterpret_cast<uint4*>(row + f0 + D / 2) = pack8(r.hi);
 }
 
-// Cosines and sines of token t at the lane's eight frequencies.  A position
-// outside the table is recorded and read as position 0.
+// Cosines and sines of token t at the lane's eight frequencies, in two steps: the
+// position is on its way with the rows and the slot, ahead of knowing whether the
+// token takes part.  A position outside the table is recorded and read as position
+// 0.  By eights: each group of eight frequencies turns by one axis, so a lane looks
+// up one position.
+__device__ __forceinline__ int load_position(const PagedAppendParams& p, int t, int f0) {
+    return p.positions[(size_t)p.axis[f0] * p.T + t];
+}
+
 template <int D>
-__device__ __forceinline__ void load_angles(const PagedAppendParams& p, int t, int f0, float (&c)[8],
-                                            float (&s)[8]) {
+__device__ __forceinline__ void load_angles(const PagedAppendParams& p, int t, int f0, int pos,
+                                            float (&c)[8], float (&s)[8]) {
     constexpr int kHalf = D / 2;
-    auto at = [&](int axis) {
-        int pos = p.positions[(size_t)axis * p.T + t];
-        if ((unsigned)pos >= (unsigned)p.table_rows) {
-            record_error(p.err, kDevBadIndex);
-            pos = 0;
-        }
-        return pos;
+    auto in_table = [&](int x) {
+        if ((unsigned)x < (unsigned)p.table_rows) return x;
+        record_error(p.err, kDevBadIndex);
+        return 0;
     };
     if (p.by_eights) {
-        const size_t e = (size_t)at(p.axis[f0]) * kHalf + f0;
+        const size_t e = (size_t)in_table(pos) * kHalf + f0;
 #pragma unroll
         for (int j = 0; j < 8; j += 4) {
             const float4 cv = *reinterpret_cast<const float4*>(p.cos_tab + e + j);
@@ -101,7 +138,7 @@ __device__ __forceinline__ void load_angles(const PagedAppendParams& p, int t, i
     }
 #pragma unroll 1
     for (int j = 0; j < 8; ++j) {
-        const size_t e = (size_t)at(p.axis[f0 + j]) * kHalf + f0 + j;
+        const size_t e = (size_t)in_table(load_position(p, t, f0 + j)) * kHalf + f0 + j;
         const float cj = p.cos_tab[e], sj = p.sin_tab[e];
 #pragma unroll
         for (int x = 0; x < 8; ++x)
@@ -231,11 +268,11 @@ struct Kv4Pages {
         }
         if (!real) return;
         const Kv4View& c = p.cache;
-        const int page = int(slot / c.page_size), row = int(slot - (long long)page * c.page_size);
-        uint8_t* dst = (which ? c.v : c.k) + c.row(page, h, row) + f0 / 2;
+        const SlotPlace at(slot, c.page_size);
+        uint8_t* dst = (which ? c.v : c.k) + c.row(at.page, h, at.row) + f0 / 2;
         *reinterpret_cast<uint32_t*>(dst) = kv4_codes(r.lo, g[0]);
         *reinterpret_cast<uint32_t*>(dst + D / 4) = kv4_codes(r.hi, g[NG - 1]);
-        __half2* pairs = c.pairs<D>(page, h, row) + which * NG;
+        __half2* pairs = c.pairs<D>(at.page, h, at.row) + which * NG;
         if (f0 == 0) {
 #pragma unroll
             for (int x = 0; x < NG; ++x) pairs[x] = g[x].bits;
@@ -246,7 +283,7 @@ struct Kv4Pages {
 // CTAs 0 .. kv_ctas - 1: rows of K (a lane group per token and kv head); as
 // many: of V; the others: kQRows query heads of a token per lane group.
 template <int D, class Pages>
-__global__ void __launch_bounds__(kPagedThreads)
+__global__ void __launch_bounds__(kPagedThreads, kPagedCtas)
 paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
     constexpr int LPR = D / 16;
     constexpr int ROWS = kPagedThreads / LPR;
@@ -259,12 +296,14 @@ paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
         const bool there = i < p.T * p.Hkv;
         const int t = there ? i / p.Hkv : 0, h = i - t * p.Hkv;
         long long slot = -1;
+        int pos = 0;
         uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if (there) {
             const __half* src = p.in[1 + which] + t * p.stride[1 + which] + (size_t)h * D + f0;
-            raw[0] = *reinterpret_cast<const uint4*>(src);
-            raw[1] = *reinterpret_cast<const uint4*>(src + D / 2);
+            raw[0] = load_row(src);
+            raw[1] = load_row(src + D / 2);
             slot = p.slots[t];
+            if (!which) pos = load_position(p, t, f0);
         }
         const bool held = slot >= 0 && slot < p.pool;
         Row16 r;
@@ -275,7 +314,7 @@ paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
             if (p.bias[1 + which]) add_bias16<D>(r, p.bias[1 + which] + (size_t)h * D, f0);
             if (!which) {
                 float c[8], s[8];
-                load_angles<D>(p, t, f0, c, s);
+                load_angles<D>(p, t, f0, pos, c, s);
                 turn16(r, c, s);
             }
             if (p.out[1 + which])
@@ -295,12 +334,14 @@ paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
 #pragma unroll
     for (int j = 0; j < kQRows; ++j)
         if (h0 + j < p.H) {
-            raw[j][0] = *reinterpret_cast<const uint4*>(src + j * D);
-            raw[j][1] = *reinterpret_cast<const uint4*>(src + j * D + D / 2);
+            raw[j][0] = load_row(src + j * D);
+            raw[j][1] = load_row(src + j * D + D / 2);
         }
-    if (p.slots[t] < 0) return;
+    const long long slot = p.slots[t];
+    const int pos = load_position(p, t, f0);
+    if (slot < 0) return;
     float c[8], s[8];
-    load_angles<D>(p, t, f0, c, s);
+    load_angles<D>(p, t, f0, pos, c, s);
     __half* dst = p.out[0] + t * p.stride[3] + (size_t)h0 * D;
 #pragma unroll
     for (int j = 0; j < kQRows; ++j)
@@ -315,61 +356,80 @@ paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Read-back: out[i] = fp16(code * scale + bias) of slot slots[i], every kv head;
-// a slot outside the pool gives zeros.  One thread widens 16 codes (an 8-byte
-// load) of K and of V, into 32 bytes each.
+// Read-back: out[i] = code * scale + bias of slot slots[i], every kv head, rounded
+// to fp16 once; a slot outside the pool gives zeros.  D / 16 lanes share a row of K
+// and V; lane l widens dims 8l .. 8l + 7 of each half row, so that every access of
+// neighbouring lanes is contiguous.
+//
+// A byte copied to both halves of a word, masked and put under 0x6400, is the fp16
+// pair 1024 + n, 1024 + 16 n'; one fused product makes n, n' of it, exactly, and a
+// second the value: code * scale is exact, so the sum is rounded once.  (Codes
+// through integer conversions and fp32, 16 a lane in two 16-byte pieces: 57 thousand
+// rows of 4 x 128, 150 MB, took 33.0 us instead of 26.1, 5.7 TB/s.)
 // ---------------------------------------------------------------------------
 struct Kv4GatherParams {
     Kv4View cache;
     const long long* slots;
     __half* k_out;
     __half* v_out;
-    long long pieces;                   // slots x Hkv x D / 16
+    uint32_t rows;                      // slots x Hkv
 };
 
-__device__ __forceinline__ void kv4_widen16(uint2 w, __half2 pair, __half* out) {
-    const float2 g = __half22float2(pair);
-    const uint32_t in[2] = {w.x, w.y};
-    uint4 h[2];
+__device__ __forceinline__ uint4 kv4_widen8(uint32_t w, uint32_t pair) {
+    const uint32_t scale = __byte_perm(pair, pair, 0x1010), bias = __byte_perm(pair, pair, 0x3232);
+    const __half2 one = __halves2half2(__ushort_as_half(0x3c00), __ushort_as_half(0x2c00));     // 1, 1/16
+    const __half2 off = __halves2half2(__ushort_as_half(0xe400), __ushort_as_half(0xd400));     // -1024, -64
+    uint32_t r[4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = fmaf(float((in[i] >> (4 * j)) & 15u), g.x, g.y);
-        h[i] = pack8(x);
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t both = (__byte_perm(w, w, i * 0x1111) & 0x00f0000fu) | 0x64006400u;
+        const __half2 n = __hfma2(*reinterpret_cast<const __half2*>(&both), one, off);
+        const __half2 x = __hfma2(n, *reinterpret_cast<const __half2*>(&scale),
+                                  *reinterpret_cast<const __half2*>(&bias));
+        r[i] = *reinterpret_cast<const uint32_t*>(&x);
     }
-    reinterpret_cast<uint4*>(out)[0] = h[0];
-    reinterpret_cast<uint4*>(out)[1] = h[1];
+    return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
 template <int D>
 __global__ void __launch_bounds__(256)
 kv4_gather_kernel(const Kv4GatherParams p) {
-    constexpr int PPR = D / 16;                 // pieces per row
+    constexpr int LPR = D / 16;                 // lanes per row
     constexpr int NG = D / kKv4Group;
     grid_launch_dependents();
     grid_dependency_wait();
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= p.pieces) return;
+    const uint32_t row = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;
+    if (row >= p.rows) return;
     const Kv4View& c = p.cache;
-    const int e = int(i % PPR) * 16;
-    const long long row = i / PPR;
-    const int h = int(row % c.Hkv);
-    const long long slot = p.slots[row / c.Hkv];
-    const bool real = slot >= 0 && slot < (long long)c.num_pages * c.page_size;
-    const int page = real ? int(slot / c.page_size) : 0;
-    const int r = real ? int(slot - (long long)page * c.page_size) : 0;
-    const __half2 zero = __halves2half2(__ushort_as_half(0), __ushort_as_half(0));
-    __half2 kp = zero, vp = zero;
-    uint2 kw = make_uint2(0, 0), vw = kw;
-    if (real) {
-        const size_t at = c.row(page, h, r) + e / 2;
-        const __half2* pairs = c.pairs<D>(page, h, r) + e / kKv4Group;
-        if (p.k_out) { kw = *reinterpret_cast<const uint2*>(c.k + at); kp = pairs[0]; }
-        if (p.v_out) { vw = *reinterpret_cast<const uint2*>(c.v + at); vp = pairs[NG]; }
+    const int l = threadIdx.x % LPR;
+    const uint32_t i = row / (uint32_t)c.Hkv;
+    const int h = row - i * c.Hkv;
+    const long long slot = p.slots[i];
+    uint32_t w[2][2] = {}, pair[2 * NG] = {};   // K's, V's two words; K's groups, V's groups
+    if (slot >= 0 && slot < (long long)c.num_pages * c.page_size) {
+        const SlotPlace at(slot, c.page_size);
+        const size_t off = c.row(at.page, h, at.row) + 4 * l;
+        const __half2* pairs = c.pairs<D>(at.page, h, at.row);
+        if constexpr (NG == 2) {
+            const uint4 x = *reinterpret_cast<const uint4*>(pairs);
+            pair[0] = x.x; pair[1] = x.y; pair[2] = x.z; pair[3] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(pairs);
+            pair[0] = x.x; pair[1] = x.y;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (p.k_out) w[0][e] = *reinterpret_cast<const uint32_t*>(c.k + off + e * (D / 4));
+            if (p.v_out) w[1][e] = *reinterpret_cast<const uint32_t*>(c.v + off + e * (D / 4));
+        }
     }
-    if (p.k_out) kv4_widen16(kw, kp, p.k_out + row * D + e);
-    if (p.v_out) kv4_widen16(vw, vp, p.v_out + row * D + e);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const size_t to = (size_t)row * D + e * (D / 2) + 8 * l;
+        const int x = NG == 2 ? e : 0;
+        if (p.k_out) *reinterpret_cast<uint4*>(p.k_out + to) = kv4_widen8(w[0][e], pair[x]);
+        if (p.v_out) *reinterpret_cast<uint4*>(p.v_out + to) = kv4_widen8(w[1][e], pair[NG + x]);
+    }
 }
 
 }  // namespace fr
