@@ -1,5 +1,5 @@
-"""A small serving loop over the 8-bit paged cache: the operators together, as a
-server calls them.
+"""A small serving loop over a paged cache in 8, 4 or 16 bits: the operators
+together, as a server calls them.
 
 Requests come with prompts of different lengths, are decoded token by token,
 end, and others start in their rows:
@@ -11,14 +11,17 @@ end, and others start in their rows:
     prefill_attn_causal   prompts, on the 16-bit K/V that the append returns
     decode_attn_paged_kv8 one token per request, on the 8-bit cache
 
+(qkv_rope_append_kv4 and decode_attn_paged_kv4 over 4 bits, qkv_rope_append_paged
+and decode_attn_paged over 16-bit pages.)
+
 A decode step (block tables, every layer's append and attention) is one CUDA
 graph, replayed while the lengths, tables and free pages move on the device.
 There are no weights: each layer's q, k, v projections are synthetic N(0, 1).
 
-Usage: python -m forgert_b200.kv8_serve [--code int8|e4m3] [--requests N]
+Usage: python -m forgert_b200.kv8_serve [--code int8|e4m3|int4|fp16] [--requests N]
        [--layers N] [--steps N]
 Prints the time of a decode step and how far the last step's attention is from
-softmax attention in 64 bits over the cache read back with kv8_gather.
+softmax attention in 64 bits over the cache read back as fp16.
 """
 from __future__ import annotations
 
@@ -28,7 +31,10 @@ import math
 
 class Server:
     """`rows` request slots over one pool of pages (shared by all layers, each
-    with a cache of its own).
+    with a cache of its own).  dtype: what the cache holds, torch.int8 or
+    torch.float8_e4m3fn codes (A.KV8Cache), torch.uint8 for codes of 4 bits
+    (A.KV4Cache), torch.float16 for the rows themselves (caches are then pairs of
+    K's and V's pages).
 
     A step's tokens are packed: token t of the step is row t of prefill's q, k
     and v.  decode's have one row per request instead, whether it takes part
@@ -61,12 +67,22 @@ class Server:
         self.row_positions = torch.zeros(rows, **i32)
         self.row_slots = torch.full((rows,), -1, dtype=torch.int64, device="cuda")
         self.cos, self.sin = A.rope_tables_device(rope_rows, head_dim, theta)
-        self.caches = [A.KV8Cache.empty(num_pages, page_size, num_kv_heads, head_dim, dtype)
-                       for _ in range(layers)]
+        self.bits = {torch.uint8: 4, torch.float16: 16}.get(dtype, 8)
+        if self.bits == 16:
+            shape = (num_pages, page_size, num_kv_heads, head_dim)
+            self.caches = [tuple(torch.empty(shape, dtype=dtype, device="cuda") for _ in range(2))
+                           for _ in range(layers)]
+        elif self.bits == 4:
+            self.caches = [A.KV4Cache.empty(num_pages, page_size, num_kv_heads, head_dim)
+                           for _ in range(layers)]
+        else:
+            self.caches = [A.KV8Cache.empty(num_pages, page_size, num_kv_heads, head_dim, dtype)
+                           for _ in range(layers)]
         # before any capture, once for good: the attention's partial states, the
         # step's counter, and what a prompt of any length splits into
+        need = {4: A.kv4_workspace_size, 8: A.kv8_workspace_size, 16: A.decode_workspace_size}[self.bits]
         A.reserve_workspace(max(
-            A.kv8_workspace_size(rows, num_heads, num_kv_heads, head_dim, max_len),
+            need(rows, num_heads, num_kv_heads, head_dim, max_len),
             max(A.prefill_workspace_size(n, num_heads, head_dim) for n in range(1, max_len + 1))))
 
     def step(self, max_tokens: int, stream=None) -> None:
@@ -94,10 +110,17 @@ class Server:
         """`tokens` rows at `positions` and `slots`, by default the packed tokens'."""
         from . import attention as A
 
-        A.qkv_rope_append_kv8(q, k, v, q_out, k_out, v_out, self.cos, self.sin,
-                              self.positions if positions is None else positions,
-                              self.slots if slots is None else slots, self.caches[layer], tokens,
-                              self.H, self.rope_rows, stream=stream)
+        positions = self.positions if positions is None else positions
+        slots = self.slots if slots is None else slots
+        args = (q, k, v, q_out, k_out, v_out, self.cos, self.sin, positions, slots)
+        cache = self.caches[layer]
+        if self.bits == 16:
+            A.qkv_rope_append_paged(*args, *cache, self.page_size, self.num_pages, tokens, self.H,
+                                    self.Hkv, self.D, self.rope_rows, stream=stream)
+        elif self.bits == 4:
+            A.qkv_rope_append_kv4(*args, cache, tokens, self.H, self.rope_rows, stream=stream)
+        else:
+            A.qkv_rope_append_kv8(*args, cache, tokens, self.H, self.rope_rows, stream=stream)
 
     def decode(self, layer: int, q, k, v, out, stream=None) -> None:
         """One layer of a step in which every request gets one token or none:
@@ -107,8 +130,15 @@ class Server:
         from . import attention as A
 
         self.append(layer, q, k, v, q, None, None, self.rows, stream, self.row_positions, self.row_slots)
-        A.decode_attn_paged_kv8(q, self.caches[layer], self.table, self.kv_lens, out, self.rows,
-                                self.H, self.width, self.max_len, stream=stream)
+        cache = self.caches[layer]
+        if self.bits == 16:
+            A.decode_attn_paged(q, *cache, self.table, self.kv_lens, out, self.rows, self.H, self.Hkv,
+                                self.D, self.page_size, self.num_pages, self.width, self.max_len,
+                                stream=stream)
+        else:
+            attn = A.decode_attn_paged_kv4 if self.bits == 4 else A.decode_attn_paged_kv8
+            attn(q, cache, self.table, self.kv_lens, out, self.rows, self.H, self.width, self.max_len,
+                 stream=stream)
 
     def prefill(self, layer: int, q, k, v, lens) -> list:
         """Prompts of the step, one after the other in q, k, v; their attention."""
@@ -138,9 +168,13 @@ def attention64(server: Server, layer: int, row: int, q):
     n = int(server.kv_lens[row])
     pos = torch.arange(n, device="cuda")
     slots = server.table[row, pos // server.page_size].long() * server.page_size + pos % server.page_size
-    k = torch.empty((n, server.Hkv, server.D), dtype=torch.float16, device="cuda")
-    v = torch.empty_like(k)
-    A.kv8_gather(server.caches[layer], slots, k, v, n)
+    cache = server.caches[layer]
+    if server.bits == 16:
+        k, v = (x.flatten(0, 1)[slots] for x in cache)
+    else:
+        k = torch.empty((n, server.Hkv, server.D), dtype=torch.float16, device="cuda")
+        v = torch.empty_like(k)
+        (A.kv4_gather if server.bits == 4 else A.kv8_gather)(cache, slots, k, v, n)
     group = server.H // server.Hkv
     k, v = (x.double().repeat_interleave(group, 1).transpose(0, 1) for x in (k, v))
     p = torch.softmax(k @ q.double()[:, :, None] / math.sqrt(server.D), 1)
@@ -160,7 +194,7 @@ def run(requests: int = 16, layers: int = 4, steps: int = 64, code: str = "int8"
     def rand(*shape):
         return torch.randn(shape, generator=gen, device="cuda", dtype=torch.float16)
 
-    dtype = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}[code]
+    dtype = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn, "int4": torch.uint8, "fp16": torch.float16}[code]
     max_len = longest + 2 * steps + 1
     s = Server(requests, num_heads, num_kv_heads, head_dim, layers, page_size,
                requests * -(-max_len // page_size), max_len, requests * longest, dtype)
@@ -232,7 +266,7 @@ def run(requests: int = 16, layers: int = 4, steps: int = 64, code: str = "int8"
 
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
-    ap.add_argument("--code", choices=("int8", "e4m3"), default="int8")
+    ap.add_argument("--code", choices=("int8", "e4m3", "int4", "fp16"), default="int8")
     ap.add_argument("--requests", type=int, default=16)
     ap.add_argument("--layers", type=int, default=4)
     ap.add_argument("--steps", type=int, default=64)
