@@ -66,7 +66,7 @@ struct DeviceState {
     int resident[4][5] = {{-1, -1, -1, -1, -1}, {-1, -1, -1, -1, -1}, {-1, -1, -1, -1, -1},
                           {-1, -1, -1, -1, -1}};   // co-resident clusters per (slot, log2 size)
     int kv8_occ[16] = {0};       // CTAs/SM of the 8-bit decode kernels (0 = not prepared)
-    int kv4_occ[8] = {0};        // ... and of the 4-bit ones
+    int kv4_occ[6] = {0};        // ... and of the 4-bit ones
     bool step_ready = false;     // paged_step_kernel's shared-memory attribute set
     int resident_g[4][2] = {{-1, -1}, {-1, -1}, {-1, -1}, {-1, -1}};   // grouped form, 8 / 16
 };

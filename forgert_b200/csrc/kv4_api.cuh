@@ -53,7 +53,8 @@ fr::Kv4View kv4_view(const fr_kv4_cache* c) {
 // of 8192 to 16384 tokens, 8 heads: 60.6 -> 54.7 us).
 //   for long calls three CTAs per SM (168 registers; at 128 for four the state
 //     spills: 64 sequences of 8192 to 32768 tokens 149 -> 246 us);
-//   DEEP, for calls of few tiles per SM: fewer CTAs, weights in two fp16 parts.
+//   DEEP, for calls of few tiles per SM: up to 8 heads, more steps under way in
+//     fewer CTAs, weights in two fp16 parts (in long calls these would cost 17 %).
 template <int D, int NT, bool DEEP> struct Kv4Shape {
     static constexpr int kMT = 2, kCtas = 2, kStages = 4;
 };
@@ -70,13 +71,10 @@ using Kv4FormatOf = fr::Kv4Format<D, NT, Kv4Shape<D, NT, DEEP>::kMT, Kv4Shape<D,
 // f(Format) for the sizes at hand.
 template <class F>
 int kv4_dispatch(int head_dim, int nt, bool deep, F f) {
-    auto with_nt = [&](auto d, auto n) {
-        constexpr int D = decltype(d)::value, NT = decltype(n)::value;
-        return deep ? f(Kv4FormatOf<D, NT, true>()) : f(Kv4FormatOf<D, NT, false>());
-    };
     auto with_d = [&](auto d) {
-        return nt == 1 ? with_nt(d, std::integral_constant<int, 1>())
-                       : with_nt(d, std::integral_constant<int, 2>());
+        constexpr int D = decltype(d)::value;
+        return deep ? f(Kv4FormatOf<D, 1, true>())
+                    : nt == 1 ? f(Kv4FormatOf<D, 1, false>()) : f(Kv4FormatOf<D, 2, false>());
     };
     return head_dim == 64 ? with_d(std::integral_constant<int, 64>())
                           : with_d(std::integral_constant<int, 128>());
@@ -86,14 +84,25 @@ int kv4_plan(DeviceState* st, int batch, int num_heads, int num_kv_heads, int he
              int max_kv_len, CachedPlan* out) {
     CachedPlan pl;
     const int group = num_heads / num_kv_heads;
-    pl.nt = group <= 8 ? 1 : 2;
-    pl.head_groups = (group + 8 * pl.nt - 1) / (8 * pl.nt);
-    pl.chunk = cached_chunk(batch, num_kv_heads, pl.head_groups, kKv4Tile, max_kv_len);
+    auto tiles_of = [&](int nt) {
+        pl.nt = nt;
+        pl.head_groups = (group + 8 * nt - 1) / (8 * nt);
+        pl.chunk = cached_chunk(batch, num_kv_heads, pl.head_groups, kKv4Tile, max_kv_len);
+        return (long long)pl.chunk * num_kv_heads * pl.head_groups *
+               std::max(1, (max_kv_len + kKv4Tile - 1) / kKv4Tile);
+    };
+    // The deep shape up to 11 tiles per SM, were every sequence as long as the
+    // longest may be (28 / 4 heads of 128, deep / long shape: 64 sequences of 200 to
+    // 300 tokens 9.8 / 10.6 us, one of 2048 9.8 / 9.7, 17 of up to 2999 with 12 / 2
+    // heads 14.1 / 13.5; 64 of 1024 to 8192 52.4 / 44.5).
+    long long tiles = tiles_of(group <= 8 ? 1 : 2);
+    pl.deep = tiles <= 11LL * st->sm_count;
+    // A second tile of 8 heads shares the codes' masks but leaves two CTAs per SM: it
+    // pays in long calls (16 / 1 heads of 128, two tiles / each by itself: 64
+    // sequences of 8192 to 16384 tokens 48.2 / 54.1 us, one of 2048 12.7 / 9.5).
+    if (pl.deep) tiles = tiles_of(1);
     if (pl.chunk <= 0) return FR_ERR_INVALID_ARG;
-    const long long tiles = (long long)pl.chunk * num_kv_heads * pl.head_groups *
-                            std::max(1, (max_kv_len + kKv4Tile - 1) / kKv4Tile);
-        pl.deep = tiles <= 11LL * st->sm_count;
-    int* occ = &st->kv4_occ[(head_dim == 64 ? 0 : 4) + (pl.nt - 1) * 2 + (pl.deep ? 1 : 0)];
+    int* occ = &st->kv4_occ[(head_dim == 64 ? 0 : 3) + (pl.deep ? 2 : pl.nt - 1)];
     int rc = kv4_dispatch(head_dim, pl.nt, pl.deep,
                           [&](auto format) { return prepare_cached<decltype(format)>(occ); });
     if (rc != FR_OK) return rc;
