@@ -49,8 +49,9 @@ fr::Kv4View kv4_view(const fr_kv4_cache* c) {
 
 // Shapes of the decode kernel: four warps, kMT blocks of 16 rows a step (what a
 // step costs beside its blocks, about 86 instructions a warp, is a seventh of the
-// two blocks' at D = 128; at D = 64 four blocks a step instead of two, 32 sequences
-// of 8192 to 16384 tokens, 8 heads: 60.6 -> 54.7 us).
+// two blocks' at D = 128; four blocks a step instead of two: 32 sequences of 8192
+// to 16384 tokens, 8 heads of 64, 60.6 -> 54.7 us, 64 of them with 16 / 1 heads of
+// 128 48.2 -> 46.1; with up to 8 heads of 128 shared memory holds two).
 //   for long calls three CTAs per SM (168 registers; at 128 for four the state
 //     spills: 64 sequences of 8192 to 32768 tokens 149 -> 246 us);
 //   DEEP, for calls of few tiles per SM: up to 8 heads, more steps under way in
@@ -58,6 +59,8 @@ fr::Kv4View kv4_view(const fr_kv4_cache* c) {
 template <int D, int NT, bool DEEP> struct Kv4Shape {
     static constexpr int kMT = 2, kCtas = 2, kStages = 4;
 };
+template <> struct Kv4Shape<128, 2, false> { static constexpr int kMT = 4, kCtas = 2, kStages = 2; };
+template <> struct Kv4Shape<64, 2, false> { static constexpr int kMT = 4, kCtas = 2, kStages = 3; };
 template <> struct Kv4Shape<128, 1, false> { static constexpr int kMT = 2, kCtas = 3, kStages = 3; };
 template <> struct Kv4Shape<64, 1, false> { static constexpr int kMT = 4, kCtas = 3, kStages = 3; };
 template <> struct Kv4Shape<64, 1, true> { static constexpr int kMT = 2, kCtas = 3, kStages = 4; };

@@ -504,7 +504,7 @@ struct Kv4Loader {
     static constexpr int RPC = LPB / CPR;       // rows of a block per warp-wide copy
     static constexpr int kRowScales = 8 * (D / kKv4Group);
     static constexpr int kTile = kBlock * MT * NW;
-    static_assert(32 % MT == 0 && kRowScales <= LPB && LPB % CPR == 0 && RPC % 2 == 0, "lanes of a block");
+    static_assert(32 % MT == 0 && LPB % CPR == 0 && RPC % 2 == 0, "lanes of a block");
     TileCursor cur;
     int idx, sub, left;                         // the lane's block: page index, block within the page, positions from there on
     int page;
@@ -565,10 +565,12 @@ struct Kv4Loader {
         };
         if (row_stride == D / 2) rows(std::integral_constant<uint32_t, D / 2>());
         else rows(row_stride);
-        if (kRowScales == LPB || lane % LPB < kRowScales) {     // 16 rows of kRowScales bytes, 16 a lane
+        if (kRowScales >= LPB || lane % LPB < kRowScales) {     // 16 rows of kRowScales bytes, 16 at a time
             const uint32_t from = scale_off + pg * p.cache.scales16 + sub * kRowScales;
-            cp_async_16(scale_at + scale_dst, reinterpret_cast<const uint8_t*>(p.cache.scales) + (size_t)from * 16,
-                        bytes, policy);
+            const uint8_t* src = reinterpret_cast<const uint8_t*>(p.cache.scales) + (size_t)from * 16;
+#pragma unroll
+            for (int i = 0; i == 0 || i * LPB < kRowScales; ++i)
+                cp_async_16(scale_at + scale_dst + i * LPB * 16, src + i * LPB * 16, bytes, policy);
         }
     }
     __device__ __forceinline__ void advance(const CachedDecodeParams<Kv4View>& p, const int* seq_start,
