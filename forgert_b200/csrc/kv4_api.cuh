@@ -42,7 +42,7 @@ fr::Kv4View kv4_view(const fr_kv4_cache* c) {
     v.row_stride = c->row_stride;
     v.page16 = (uint32_t)(c->page_stride / 16);
     v.block16 = (uint32_t)c->row_stride;
-    v.head_scales16 = (uint32_t)(c->page_size * (c->head_dim / 8) / 16);
+    v.head_scales16 = (uint32_t)((long long)c->page_size * (c->head_dim / 8) / 16);
     v.scales16 = c->num_kv_heads * v.head_scales16;
     return v;
 }

@@ -22,9 +22,15 @@
 // group's reference, in fp32 from unrounded p.
 //
 // Bytes: D of codes per position and kv head, D / 8 of scales; 4 * D * G
-// operations on them.  At D = 128 a block of 16 positions and one kv head takes a
-// warp about 287 instructions, 124 of them on the integer pipe, which takes one in
-// two cycles: 80 masks and shifts of codes (5 for 8 codes), 18 products.
+// operations on them.  Measured, 28 / 4 heads of 128: 64 sequences of 8192 to 32768
+// tokens (1.2 million tokens, 697 MB) 147 us, 4.7 TB/s, 0.72 of a copy's rate; of
+// 1024 to 8192 45 us; one sequence of 512 tokens 7.4 (14 / 2 heads of 64).  Bound by
+// the warps' instructions: the copies alone take 106 and 32 us.  At D = 128 a block
+// of 16 positions and one kv head takes a warp about 290, 124 of them on the integer
+// pipe, which takes one in two cycles: 80 masks and shifts of codes (5 for 8
+// codes), beside 18 products of 8 cycles each; 43 are a half of a step's overhead.
+// Twelve warps per SM issue in 55 to 59 % of the cycles whatever the order of the
+// phases (scores of two blocks at once, V loaded early or late: within 1 %).
 //
 // Fragments (mma m16n8k16): of K a lane holds 16 dims of each group in rows 2g and
 // 2g + 1 of the block, as they lie in memory; contraction order is free, so q is

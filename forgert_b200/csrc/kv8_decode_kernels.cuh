@@ -24,14 +24,9 @@
 // per SM) and latency, about 7 us of them launch, first rows, fold and merge;
 // one sequence of 512 tokens 8 (14 / 2 heads of 64).
 //
-// Decomposition: persistent CTAs take equal shares of the batch's work, as in
-// batched_kernels.cuh (units, items, pieces merged by the contributor that
-// completes a unit), over tiles of TILE = 16 * MT * NW positions.  Inside a
-// CTA every warp streams for itself: warp w copies and consumes rows
-// 16 * MT * w .. of each tile through a ring of its own (cp.async, STAGES
-// steps of MT blocks of K and V and their scales), so a step needs no barrier
-// between warps and no producer, and any strides and page size will do.  The
-// page of a step is looked up one step before its copies start.
+// Decomposition: the frame's (cached_decode_kernels.cuh).  A warp's copies are
+// cp.async, so any strides and page size will do.  The page of a step is looked up
+// one step before its copies start.
 // (Copies by TMA boxes of gcd(page_size, TILE) rows, one producer warp per
 // CTA, were measured first: with pages of 16 rows the boxes of 2 KB took 80 ns
 // each, 95 us for 304 MB, where pages of 64 rows took 64 us for 272 MB.)
