@@ -141,11 +141,17 @@ int run_kv4(const void* q, long long q_stride, const fr_kv4_cache* cache, const 
     p.max_units = kCachedUnits;
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(st->ws) + kCounterBytes);
     p.part_acc = p.part_ml + (size_t)2 * pl.ctas * 8 * pl.nt * 2;
-    p.min_tiles_per_cta = 2;
+    // One tile per CTA is enough before SMs get more than one (two: 17 sequences of
+    // up to 2999 tokens, 12 / 2 heads of 128, 14.0 us instead of 11.8, no call
+    // measured faster).  A unit's start and its merge are charged as one tile each
+    // (none: 64 sequences of 1024 to 8192 45.5 -> 47.4, one of 512 7.4 -> 6.8; two:
+    // 46.4 and 8.0), and units of up to four tiles are not cut (one of 512 7.4 ->
+    // 7.1, 64 of 200 to 300 15.7 -> 9.9; six: one of 640 8.8 -> 10.1).
+    p.min_tiles_per_cta = 1;
     p.min_ctas = st->sm_count;
     p.item_cost = 1;
     p.merge_cost = 1;
-    p.whole_tiles = 3;
+    p.whole_tiles = 4;
     for (int b = 0; b < batch; b += pl.chunk) {
         p.batch = std::min(pl.chunk, batch - b);
         p.q = static_cast<const __half*>(q) + (size_t)b * q_stride;
