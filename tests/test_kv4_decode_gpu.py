@@ -65,6 +65,10 @@ def to_cache(kc, vc, scales, layout="head"):
         x = torch.from_numpy(c).cuda()
         if layout == "token":                          # [P, ps, Hkv, D / 2] pages
             x = x.transpose(1, 2).contiguous().transpose(1, 2)
+        if layout == "heads":                          # [Hkv, P, ps, D / 2]
+            x = x.transpose(0, 1).contiguous().transpose(0, 1)
+        if layout == "padded":                         # rows 16 bytes apart
+            x = torch.cat([x, torch.full_like(x[..., :16], 255)], -1)[..., :x.shape[-1]]
         return x
     if layout == "mixed":                              # K and V pages side by side in one allocation
         both = torch.stack([torch.from_numpy(kc), torch.from_numpy(vc)], 1).cuda()
@@ -171,6 +175,22 @@ def test_strides(layout, H, Hkv, D):
     got = run(q, to_cache(kc, vc, scales, layout), table, lens, q_stride=wide.stride(0), qd=wide)
     check(got, q, kc, vc, scales, table, lens)
     assert np.array_equal(got, run(q, to_cache(kc, vc, scales), table, lens))
+
+
+@pytest.mark.parametrize("layout", ["token", "mixed", "heads", "padded"])
+@pytest.mark.parametrize("H,Hkv,D", [(14, 2, 64), (24, 2, 64), (28, 4, 128), (16, 1, 128)])
+def test_strides_long(layout, H, Hkv, D):
+    """The shapes for long calls on every layout: the bits are those of the plain one."""
+    rng = np.random.default_rng(16)
+    lens = [77, 0, 1640, 33]
+    q = half(rng, (4, H, D))
+    table, pages = make_table(rng, lens, 48)
+    kc, vc, scales = make_pool(rng, pages, Hkv, 48, D)
+    got = run_long(q, to_cache(kc, vc, scales, layout), table, lens, 48)
+    check(got, q, kc, vc, scales, table, lens, long=True)
+    assert np.array_equal(got, run_long(q, to_cache(kc, vc, scales), table, lens, 48))
+    short = run(q, to_cache(kc, vc, scales, layout), table, lens)
+    check(short, q, kc, vc, scales, table, lens)
 
 
 def test_one_page_pool_and_one_head():
