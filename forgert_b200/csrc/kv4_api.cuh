@@ -96,8 +96,8 @@ int kv4_plan(DeviceState* st, int batch, int num_heads, int num_kv_heads, int he
     };
     // The deep shape up to 11 tiles per SM, were every sequence as long as the
     // longest may be (28 / 4 heads of 128, deep / long shape: 64 sequences of 200 to
-    // 300 tokens 9.8 / 10.6 us, one of 2048 9.8 / 9.7, 17 of up to 2999 with 12 / 2
-    // heads 14.1 / 13.5; 64 of 1024 to 8192 52.4 / 44.5).
+    // 300 tokens 9.9 / 10.9 us, 17 of up to 2999 with 12 / 2 heads 11.7 / 12.8, one of
+    // 2048 9.8 / 9.7, 32 of 1000 to 1500 17.9 / 17.2, 64 of 1024 to 8192 52.9 / 45.4).
     long long tiles = tiles_of(group <= 8 ? 1 : 2);
     pl.deep = tiles <= 11LL * st->sm_count;
     // A second tile of 8 heads shares the codes' masks but leaves two CTAs per SM: it
