@@ -274,6 +274,10 @@ struct Kv4Block {
     static __device__ __forceinline__ float2 wide(uint32_t h) {
         return __half22float2(*reinterpret_cast<const __half2*>(&h));
     }
+    // A sum of weights that does not fit.  NaN counts: an infinite p at a scale of 0
+    // gives one, and so does a NaN scale, beside which another group's weights may be
+    // infinite.
+    static __device__ __forceinline__ bool outgrown(float sum) { return !(sum <= kKv4Most); }
 
     // TAIL: only the first `valid` (>= 1) rows are positions.
     template <bool TAIL>
@@ -348,8 +352,9 @@ struct Kv4Block {
     }
 
     // Probabilities, their sums, and the weights P^T a' as fp16.  Where the weights
-    // of a column's rows here sum up to 2^15 or more (in fp32, on a pipe with room;
-    // with p as weights of the least scale among them), the column's references move.
+    // of a column's rows here sum up to more than 2^15 or to NaN (in fp32, on a pipe
+    // with room; with p as weights of the least scale among them), the column's
+    // references move, by the scores and finite scales alone: p is finite then.
     // ADDED: z holds what o does since it was last centred, and moves with it.
     template <bool ADDED>
     __device__ __forceinline__ void weigh(const Kv4Query<D, NT>& q, Kv4State<D, NT>& st,
@@ -388,7 +393,7 @@ struct Kv4Block {
                             rest[x][nt][i] = pack_half2(w0 - r.x, w1 - r.y);
                         }
                     }
-                over |= fmaxf(all[nt][0], all[nt][1]) > kKv4Most;
+                over |= outgrown(max_nan(all[nt][0], all[nt][1]));
             }
         };
         form();
@@ -400,7 +405,7 @@ struct Kv4Block {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const uint32_t column = 0x11111111u << (lane & 3);
-                    const bool move = st.fresh || (__ballot_sync(0xffffffffu, all[nt][j] > kKv4Most) & column);
+                    const bool move = st.fresh || (__ballot_sync(0xffffffffu, outgrown(all[nt][j])) & column);
                     const float r0 = st.r[nt][j];
                     float by0 = 0.f;
 #pragma unroll

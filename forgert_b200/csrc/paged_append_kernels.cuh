@@ -179,18 +179,6 @@ struct HalfPages {
 };
 
 // --------------------------------------------------------------------- 4 bits
-// Minima and maxima that are NaN if an operand is.
-__device__ __forceinline__ float min_nan(float a, float b) {
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-
 struct Kv4Pair {
     float scale, bias, inverse;
     __half2 bits;
