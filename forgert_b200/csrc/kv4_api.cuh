@@ -50,12 +50,15 @@ fr::Kv4View kv4_view(const fr_kv4_cache* c) {
 // Shapes of the decode kernel: four warps, kMT blocks of 16 rows a step (what a
 // step costs beside its blocks, about 86 instructions a warp, is a seventh of the
 // two blocks' at D = 128; four blocks a step instead of two: 32 sequences of 8192
-// to 16384 tokens, 8 heads of 64, 60.6 -> 54.7 us, 64 of them with 16 / 1 heads of
-// 128 48.2 -> 46.1; with up to 8 heads of 128 shared memory holds two).
-//   for long calls three CTAs per SM (168 registers; at 128 for four the state
-//     spills: 64 sequences of 8192 to 32768 tokens 149 -> 246 us);
-//   DEEP, for calls of few tiles per SM: up to 8 heads, more steps under way in
-//     fewer CTAs, weights in two fp16 parts (in long calls these would cost 17 %).
+// to 16384 tokens, 8 heads of 64, 69.4 -> 61.3 us; with up to 8 heads of 128 shared
+// memory holds two).
+//   for long calls three CTAs per SM with up to 8 heads (168 registers at D = 128,
+//     165 at 64; at 128 for four the state spills: 64 sequences of 8192 to 32768
+//     tokens 149 -> 246 us, with weights in one fp16), two with 16 (255 and 229; at
+//     D = 128 60 bytes are spilled, with two blocks a step 40, which is no faster:
+//     64 sequences of 8192 to 16384 tokens 56.1 and 56.6 us);
+//   DEEP, for calls of few tiles per SM: up to 8 heads, more steps under way (212
+//     registers at D = 128, 155 at 64).
 template <int D, int NT, bool DEEP> struct Kv4Shape {
     static constexpr int kMT = 2, kCtas = 2, kStages = 4;
 };
@@ -69,7 +72,7 @@ constexpr int kKv4Tile = 16 * 2 * kKv4Warps;    // the least of any shape: tiles
 
 template <int D, int NT, bool DEEP>
 using Kv4FormatOf = fr::Kv4Format<D, NT, Kv4Shape<D, NT, DEEP>::kMT, Kv4Shape<D, NT, DEEP>::kStages,
-                                  kKv4Warps, Kv4Shape<D, NT, DEEP>::kCtas, DEEP>;
+                                  kKv4Warps, Kv4Shape<D, NT, DEEP>::kCtas>;
 
 // f(Format) for the sizes at hand.
 template <class F>
@@ -96,13 +99,14 @@ int kv4_plan(DeviceState* st, int batch, int num_heads, int num_kv_heads, int he
     };
     // The deep shape up to 11 tiles per SM, were every sequence as long as the
     // longest may be (28 / 4 heads of 128, deep / long shape: 64 sequences of 200 to
-    // 300 tokens 9.9 / 10.9 us, 17 of up to 2999 with 12 / 2 heads 11.7 / 12.8, one of
-    // 2048 9.8 / 9.7, 32 of 1000 to 1500 17.9 / 17.2, 64 of 1024 to 8192 52.9 / 45.4).
+    // 300 tokens 9.9 / 11.4 us, 17 of up to 2999 with 12 / 2 heads 11.6 / 13.2, one of
+    // 2048 9.8 / 9.9, 32 of 1000 to 1500 17.9 / 17.9, 64 of 1024 to 8192 52.9 / 50.8;
+    // 32 of 8192 to 16384 with 8 heads of 64 69.4 / 61.3).
     long long tiles = tiles_of(group <= 8 ? 1 : 2);
     pl.deep = tiles <= 11LL * st->sm_count;
     // A second tile of 8 heads shares the codes' masks but leaves two CTAs per SM: it
     // pays in long calls (16 / 1 heads of 128, two tiles / each by itself: 64
-    // sequences of 8192 to 16384 tokens 48.2 / 54.1 us, one of 2048 12.7 / 9.5).
+    // sequences of 8192 to 16384 tokens 56.1 / 61.0 us, one of 2048 14.6 / 9.5).
     if (pl.deep) tiles = tiles_of(1);
     if (pl.chunk <= 0) return FR_ERR_INVALID_ARG;
     int* occ = &st->kv4_occ[(head_dim == 64 ? 0 : 3) + (pl.deep ? 2 : pl.nt - 1)];

@@ -9,17 +9,15 @@
 // fp16 with bits n is n 2^-24 exactly, so a mask makes two operands of a word,
 // n of the low halves and 16 n of the high ones, and the factors are taken off
 // the sums.  15 times the sum of a step's weights comes from a product with a
-// constant operand (z), and half of it is taken off o: what rounding a weight to
-// fp16 takes off then counts by the distance from the group's middle, not from its
-// bottom (half the error), and o stays small, so that its sums lose little (taken
-// off once at the end, outputs over 131072 positions were off by 3.2e-4 of their
-// 2-norm instead of 3.1e-4).  Scores, l, o and all other sums are fp32.
+// constant operand (z), and half of it is taken off o, which so stays small and its
+// sums lose little.  Scores, l, o and all other sums are fp32.
 //
-// A weight p a' enters the product with V as fp16 on a reference of its own
-// group's, 2^8 up, so that one as small as 2^-22 of the largest keeps all its
-// bits; REST adds a second product with what the rounding takes off (short calls,
-// where the outputs average fewer terms).  l and the middles are on the first
-// group's reference, in fp32 from unrounded p.
+// A weight p a' enters the product with V as two fp16, itself rounded and what the
+// rounding takes off, on a reference of its own group's, 2^8 up, so that one as
+// small as 2^-22 of the largest keeps its bits.  (One fp16 alone: 64 sequences of
+// 8192 to 32768 tokens in 147 us instead of 170, but the outputs off by 3.0e-4 of
+// their 2-norm instead of 2.1e-4, which is what their rounding takes.)  l and the
+// middles are on the first group's reference, in fp32 from unrounded p.
 //
 // Bytes: D of codes per position and kv head, D / 8 of scales; 4 * D * G
 // operations on them.  Measured, 28 / 4 heads of 128: 64 sequences of 8192 to 32768
@@ -264,7 +262,7 @@ struct Kv4Lane {
 
 // A block of 16 rows on its way through a warp: scores, weights, then the products
 // with V.
-template <int D, int NT, bool REST>
+template <int D, int NT>
 struct Kv4Block {
     static constexpr int NG = D / kKv4Group;
     float s[NT][4];                             // scores, in units of q.unit
@@ -387,11 +385,9 @@ struct Kv4Block {
                         all[nt][0] += w0;
                         all[nt][1] += w1;
                         const uint32_t h = pack_half2(w0, w1);
+                        const float2 r = wide(h);
                         w[x][nt][i] = h;
-                        if constexpr (REST) {
-                            const float2 r = wide(h);
-                            rest[x][nt][i] = pack_half2(w0 - r.x, w1 - r.y);
-                        }
+                        rest[x][nt][i] = pack_half2(w0 - r.x, w1 - r.y);
                     }
                 over |= outgrown(max_nan(all[nt][0], all[nt][1]));
             }
@@ -472,22 +468,19 @@ struct Kv4Block {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     wb[nt][i] = movmatrix_trans(w[x][nt][i]);
-                    if constexpr (REST) wr[nt][i] = movmatrix_trans(rest[x][nt][i]);
+                    wr[nt][i] = movmatrix_trans(rest[x][nt][i]);
                 }
             auto product = [&](float (&acc)[NT][4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt], a0, a1, a2, a3, wb[nt][0], wb[nt][1]);
-                if constexpr (REST) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt], a0, a1, a2, a3, wr[nt][0], wr[nt][1]);
-                }
+                for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt], a0, a1, a2, a3, wr[nt][0], wr[nt][1]);
             };
             if constexpr (FIRST) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     mma_16816_first(z[x][nt], kFifteen, kFifteen, kFifteen, kFifteen, wb[nt][0], wb[nt][1]);
-                    if constexpr (REST)
-                        mma_16816(z[x][nt], kFifteen, kFifteen, kFifteen, kFifteen, wr[nt][0], wr[nt][1]);
+                    mma_16816(z[x][nt], kFifteen, kFifteen, kFifteen, kFifteen, wr[nt][0], wr[nt][1]);
                 }
             } else {
                 product(z[x], kFifteen, kFifteen, kFifteen, kFifteen);
@@ -598,8 +591,8 @@ struct Kv4Loader {
     }
 };
 
-// Steps of MT blocks of 16 rows; CTAS per SM; REST as above.
-template <int D, int NT, int MT, int STAGES, int NW, int CTAS, bool REST>
+// Steps of MT blocks of 16 rows; CTAS per SM.
+template <int D, int NT, int MT, int STAGES, int NW, int CTAS>
 struct Kv4Format {
     static constexpr int kD = D, kNT = NT, kMT = MT, kStages = STAGES, kNW = NW, kCtas = CTAS, kRun = 1;
     using Params = CachedDecodeParams<Kv4View>;
@@ -618,7 +611,7 @@ struct Kv4Format {
         float z[D / kKv4Group][NT][4];
         if (valid >= 16 * MT) {
             // The next block's scores beside the products of the one before it.
-            Kv4Block<D, NT, REST> b[2];
+            Kv4Block<D, NT> b[2];
             b[0].template score<false>(at, 0, 16, q, lane);
             b[0].template weigh<false>(q, st, z, lane);
 #pragma unroll
@@ -633,7 +626,7 @@ struct Kv4Format {
         } else {
 #pragma unroll 1
             for (int i = 0; i * 16 < valid; ++i) {
-                Kv4Block<D, NT, REST> b;
+                Kv4Block<D, NT> b;
                 b.template score<true>(at, i, valid - i * 16, q, lane);
                 b.template weigh<false>(q, st, z, lane);
                 b.template apply<true>(at, i, st, z);

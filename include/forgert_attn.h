@@ -464,14 +464,10 @@ FR_API int fr_kv4_gather(const fr_kv4_cache* cache, const long long* slots, void
 /* Decode attention over the 4-bit paged cache, one token per sequence;
  * fr_decode_attn_paged_kv8's arguments.  Rows past a sequence's end are never
  * used, whatever they hold.  A NaN scale or bias of a used row makes the outputs
- * it enters NaN.  Scores and sums are fp32.  A short call is off by the rounding
- * of its outputs; a long one also rounds each weight (a probability times V's
- * scale) to fp16, 2^-11 of itself, which counts by the value's distance from the
- * middle of its group.  A call is long when batch * num_kv_heads sequences of
- * max_kv_len, in tiles of 128 positions (once more for each 16 query heads of a
- * group above 16), make more than 11 tiles per SM, at most 512 sequences
- * counted.  The result does not depend on which CTA merges: equal inputs give
- * equal bits. */
+ * it enters NaN.  Scores and sums are fp32, weights (a probability times V's
+ * scale) keep 22 bits: a call is off by the rounding of its outputs and hardly
+ * more, whatever max_kv_len.  The result does not depend on which CTA merges:
+ * equal inputs give equal bits. */
 FR_API int fr_decode_attn_paged_kv4(const void* q, long long q_stride, const fr_kv4_cache* cache,
                                     const int* block_table, const int* kv_lens, void* out,
                                     int batch, int num_heads, int max_blocks_per_seq,
