@@ -19,6 +19,7 @@
 //   Loader         init, look_up, copy, advance (cursor and pages of a warp)
 //   Query, State   q in registers; the running (m, l, o) of an item
 //   consume        one step
+//   pack           two outputs as fp16
 //   dim(dm, g)     first of the two dims that lane group g holds in fragment
 //                  dm of o; kRun (4 or 1) neighbouring dm are consecutive dims
 #pragma once
@@ -208,10 +209,10 @@ __device__ __forceinline__ void cached_merge(const typename F::Params& p, float*
         const int h = ha[i];
         if (h < gcount)
             *reinterpret_cast<uint32_t*>(p.out + (head_base + h) * D + dim) =
-                pack_half2(acc[i].x * sm_inv[h], acc[i].z * sm_inv[h]);
+                F::pack(acc[i].x * sm_inv[h], acc[i].z * sm_inv[h]);
         if (h + 1 < gcount)
             *reinterpret_cast<uint32_t*>(p.out + (head_base + h + 1) * D + dim) =
-                pack_half2(acc[i].y * sm_inv[h + 1], acc[i].w * sm_inv[h + 1]);
+                F::pack(acc[i].y * sm_inv[h + 1], acc[i].w * sm_inv[h + 1]);
     }
 }
 
@@ -373,7 +374,7 @@ cached_decode_kernel(const __grid_constant__ typename F::Params p) {
                                 uint32_t h[F::kRun];
 #pragma unroll
                                 for (int x = 0; x < F::kRun; ++x)
-                                    h[x] = pack_half2(st.o[dm + x][nt][jj] * inv, st.o[dm + x][nt][jj + 2] * inv);
+                                    h[x] = F::pack(st.o[dm + x][nt][jj] * inv, st.o[dm + x][nt][jj + 2] * inv);
                                 if constexpr (F::kRun == 4)
                                     *reinterpret_cast<uint4*>(dst + F::dim(dm, g)) = make_uint4(h[0], h[1], h[2], h[3]);
                                 else

@@ -14,6 +14,10 @@
 namespace fr {
 
 constexpr int kKv4Group = 64;                   // dims that share a scale and a bias
+// The largest fp16.  A scale is rounded up, so 15 of them above a bias may stand for
+// more than a group's maximum, and for more than this: cut where a value or an
+// average of values becomes fp16.  (Nothing lies below -65504: no bias does.)
+constexpr float kKv4Top = 65504.f;
 
 struct Kv4View {
     uint8_t* k;

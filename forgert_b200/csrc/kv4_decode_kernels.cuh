@@ -604,6 +604,9 @@ struct Kv4Format {
     static __device__ __forceinline__ int dim(int dm, int g) {
         return (dm >> 2) * kKv4Group + 16 * (dm & 3) + 2 * g;
     }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        return pack_half2(min_nan(lo, kKv4Top), min_nan(hi, kKv4Top));
+    }
     static __device__ __forceinline__ void consume(uint32_t kst, uint32_t vst, const unsigned char* sc,
                                                    int valid, const Query& q, State& st, float,
                                                    int lane) {

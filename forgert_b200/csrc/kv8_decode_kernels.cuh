@@ -448,6 +448,7 @@ struct Kv8Format {
     using State = Kv8State<D, NT>;
 
     static __device__ __forceinline__ int dim(int dm, int g) { return (D / 8) * g + 2 * dm; }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_half2(lo, hi); }
     static __device__ __forceinline__ void consume(uint32_t kst, uint32_t vst, const unsigned char* sc,
                                                    int valid, const Query& q, State& st, float sl2,
                                                    int lane) {

@@ -345,9 +345,9 @@ paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
 
 // ---------------------------------------------------------------------------
 // Read-back: out[i] = code * scale + bias of slot slots[i], every kv head, rounded
-// to fp16 once; a slot outside the pool gives zeros.  D / 16 lanes share a row of K
-// and V; lane l widens dims 8l .. 8l + 7 of each half row, so that every access of
-// neighbouring lanes is contiguous.
+// to fp16 once (65504 at most); a slot outside the pool gives zeros.  D / 16 lanes
+// share a row of K and V; lane l widens dims 8l .. 8l + 7 of each half row, so that
+// every access of neighbouring lanes is contiguous.
 //
 // A byte copied to both halves of a word, masked and put under 0x6400, is the fp16
 // pair 1024 + n, 1024 + 16 n'; one fused product makes n, n' of it, exactly, and a
@@ -367,13 +367,14 @@ __device__ __forceinline__ uint4 kv4_widen8(uint32_t w, uint32_t pair) {
     const uint32_t scale = __byte_perm(pair, pair, 0x1010), bias = __byte_perm(pair, pair, 0x3232);
     const __half2 one = __halves2half2(__ushort_as_half(0x3c00), __ushort_as_half(0x2c00));     // 1, 1/16
     const __half2 off = __halves2half2(__ushort_as_half(0xe400), __ushort_as_half(0xd400));     // -1024, -64
+    const __half2 top = __float2half2_rn(kKv4Top);
     uint32_t r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t both = (__byte_perm(w, w, i * 0x1111) & 0x00f0000fu) | 0x64006400u;
         const __half2 n = __hfma2(*reinterpret_cast<const __half2*>(&both), one, off);
-        const __half2 x = __hfma2(n, *reinterpret_cast<const __half2*>(&scale),
-                                  *reinterpret_cast<const __half2*>(&bias));
+        const __half2 x = __hmin2_nan(__hfma2(n, *reinterpret_cast<const __half2*>(&scale),
+                                              *reinterpret_cast<const __half2*>(&bias)), top);
         r[i] = *reinterpret_cast<const uint32_t*>(&x);
     }
     return make_uint4(r[0], r[1], r[2], r[3]);

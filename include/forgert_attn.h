@@ -444,9 +444,11 @@ typedef struct fr_kv4_cache {
  *   bias  = the largest fp16 number not above the group's minimum
  *   scale = the smallest fp16 number not below (maximum - bias) / 15
  *   code  = (x - bias) / scale to the nearest, ties to even (0 if scale is 0)
- * so that no value is cut off and each is off by half a scale at most.  A group
- * that holds a NaN, an infinity or a value below -65504 gets NaN for both and
- * reads back as NaN; no row's codes depend on another row. */
+ * so that no code is cut off and each value is off by half a scale at most (one
+ * that stands for more than 65504, as a scale rounded up or a bias can make it,
+ * is read as 65504).  A group that holds a NaN, an infinity or a value below
+ * -65504 gets NaN for both and reads back as NaN; no row's codes depend on
+ * another row. */
 FR_API int fr_qkv_rope_append_kv4(const void* q, const void* k, const void* v, void* q_out,
                                   void* k_out, void* v_out, const long long* token_strides,
                                   const void* q_bias, const void* k_bias, const void* v_bias,
@@ -457,17 +459,18 @@ FR_API int fr_qkv_rope_append_kv4(const void* q, const void* k, const void* v, v
                                   void* stream);
 
 /* Reads slots back as fp16: k_out, v_out [num_slots, num_kv_heads, head_dim]
- * (16-byte aligned; either may be NULL).  A slot outside the pool gives zeros. */
+ * (16-byte aligned; either may be NULL), 65504 at most.  A slot outside the pool
+ * gives zeros. */
 FR_API int fr_kv4_gather(const fr_kv4_cache* cache, const long long* slots, void* k_out,
                          void* v_out, int num_slots, void* stream);
 
 /* Decode attention over the 4-bit paged cache, one token per sequence;
  * fr_decode_attn_paged_kv8's arguments.  Rows past a sequence's end are never
  * used, whatever they hold.  A NaN scale or bias of a used row makes the outputs
- * it enters NaN.  Scores and sums are fp32, weights (a probability times V's
- * scale) keep 22 bits: a call is off by the rounding of its outputs and hardly
- * more, whatever max_kv_len.  The result does not depend on which CTA merges:
- * equal inputs give equal bits. */
+ * it enters NaN; outputs are 65504 at most.  Scores and sums are fp32, weights (a
+ * probability times V's scale) keep 22 bits: a call is off by the rounding of its
+ * outputs and hardly more, whatever max_kv_len.  The result does not depend on
+ * which CTA merges: equal inputs give equal bits. */
 FR_API int fr_decode_attn_paged_kv4(const void* q, long long q_stride, const fr_kv4_cache* cache,
                                     const int* block_table, const int* kv_lens, void* out,
                                     int batch, int num_heads, int max_blocks_per_seq,
