@@ -49,20 +49,20 @@ fr::Kv4View kv4_view(const fr_kv4_cache* c) {
 
 // Shapes of the decode kernel: four warps, kMT blocks of 16 rows a step (what a
 // step costs beside its blocks, about 86 instructions a warp, is a seventh of the
-// two blocks' at D = 128; four blocks a step instead of two: 32 sequences of 8192
-// to 16384 tokens, 8 heads of 64, 69.4 -> 61.3 us; with up to 8 heads of 128 shared
-// memory holds two).
+// two blocks' at D = 128; four blocks a step instead of two at D = 64: 32 sequences
+// of 8192 to 16384 tokens, 8 heads, 69.4 -> 61.3 us, 64 with 24 / 2 61.6 -> 55.5;
+// at D = 128 shared memory holds two with up to 8 heads, and with 16 four are as
+// fast: 64 sequences of 8192 to 16384 tokens, 16 / 1 heads, 57.8 and 57.6 us, of
+// 1024 to 8192 31.4 and 32.5).
 //   for long calls three CTAs per SM with up to 8 heads (168 registers at D = 128,
-//     165 at 64; at 128 for four the state spills: 64 sequences of 8192 to 32768
-//     tokens 149 -> 246 us, with weights in one fp16), two with 16 (255 and 229; at
-//     D = 128 60 bytes are spilled, with two blocks a step 40, which is no faster:
-//     64 sequences of 8192 to 16384 tokens 56.1 and 56.6 us);
-//   DEEP, for calls of few tiles per SM: up to 8 heads, more steps under way (212
+//     161 at 64; at 128 for four the state spills: 64 sequences of 8192 to 32768
+//     tokens 149 -> 246 us, with weights in one fp16), two with 16 (255, of which
+//     16 bytes are spilled, and 227);
+//   DEEP, for calls of few tiles per SM: up to 8 heads, more steps under way (211
 //     registers at D = 128, 155 at 64).
 template <int D, int NT, bool DEEP> struct Kv4Shape {
     static constexpr int kMT = 2, kCtas = 2, kStages = 4;
 };
-template <> struct Kv4Shape<128, 2, false> { static constexpr int kMT = 4, kCtas = 2, kStages = 2; };
 template <> struct Kv4Shape<64, 2, false> { static constexpr int kMT = 4, kCtas = 2, kStages = 3; };
 template <> struct Kv4Shape<128, 1, false> { static constexpr int kMT = 2, kCtas = 3, kStages = 3; };
 template <> struct Kv4Shape<64, 1, false> { static constexpr int kMT = 4, kCtas = 3, kStages = 3; };
@@ -106,7 +106,7 @@ int kv4_plan(DeviceState* st, int batch, int num_heads, int num_kv_heads, int he
     pl.deep = tiles <= 11LL * st->sm_count;
     // A second tile of 8 heads shares the codes' masks but leaves two CTAs per SM: it
     // pays in long calls (16 / 1 heads of 128, two tiles / each by itself: 64
-    // sequences of 8192 to 16384 tokens 56.1 / 61.0 us, one of 2048 14.6 / 9.5).
+    // sequences of 8192 to 16384 tokens 57.8 / 61.4 us, one of 2048 14.6 / 9.5).
     if (pl.deep) tiles = tiles_of(1);
     if (pl.chunk <= 0) return FR_ERR_INVALID_ARG;
     int* occ = &st->kv4_occ[(head_dim == 64 ? 0 : 3) + (pl.deep ? 2 : pl.nt - 1)];

@@ -45,6 +45,7 @@ namespace fr {
 constexpr float kKv4Shift = 8.f;        // a weight at its reference counts 2^8 ...
 constexpr float kKv4Most = 0x1p15f;     // ... and the weights of a lane's rows may sum up to 2^15 before that moves
 constexpr float kKv4Least = -24.f;      // a smaller scale's reference is this scale's: p stays below 2^39
+constexpr float kKv4Far = 0x1p23f;      // from here on scores are whole numbers
 constexpr uint32_t kLowHalves = 0x000f000fu, kHighHalves = 0x00f000f0u;
 
 // A block (16 rows) in shared memory: lines of 128 bytes, of 2 rows (D = 128) or 4,
@@ -265,7 +266,7 @@ struct Kv4Lane {
 template <int D, int NT>
 struct Kv4Block {
     static constexpr int NG = D / kKv4Group;
-    float s[NT][4];                             // scores, in units of q.unit
+    float s[NT][4];                             // scores, in base 2
     float va[2][NG], vm[2][NG];                 // V's scales and middles of the lane's rows
     uint32_t w[NG][NT][2], rest[NG][NT][2];     // weights, and what their rounding took off
 
@@ -337,7 +338,7 @@ struct Kv4Block {
                         if (x) sum = fmaf(k[x].y, q.sum[x][nt][j], sum);
                         sum = fmaf(k[x].x, d[x][nt][2 * i + j], sum);
                     }
-                    s[nt][2 * i + j] = sum;
+                    s[nt][2 * i + j] = __fmul_rn(sum, q.unit[nt][j]);
                 }
             // What rows past the end hold is anything, a NaN included.
             if (TAIL && (lane >> 2) * 2 + i >= valid) {
@@ -355,8 +356,7 @@ struct Kv4Block {
     // references move, by the scores and finite scales alone: p is finite then.
     // ADDED: z holds what o does since it was last centred, and moves with it.
     template <bool ADDED>
-    __device__ __forceinline__ void weigh(const Kv4Query<D, NT>& q, Kv4State<D, NT>& st,
-                                          float (&z)[NG][NT][4], int lane) {
+    __device__ __forceinline__ void weigh(Kv4State<D, NT>& st, float (&z)[NG][NT][4], int lane) {
         float p[NT][4], ps[NT][2], all[NT][2];
         bool over = false;
         auto form = [&]() {
@@ -365,7 +365,7 @@ struct Kv4Block {
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    p[nt][c] = fast_exp2(fmaf(s[nt][c], q.unit[nt][c & 1], -st.r[nt][c & 1]));
+                    p[nt][c] = fast_exp2(s[nt][c] - st.r[nt][c & 1]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     ps[nt][j] = p[nt][j] + p[nt][2 + j];
@@ -402,22 +402,30 @@ struct Kv4Block {
                 for (int j = 0; j < 2; ++j) {
                     const uint32_t column = 0x11111111u << (lane & 3);
                     const bool move = st.fresh || (__ballot_sync(0xffffffffu, outgrown(all[nt][j])) & column);
+                    // Scores so large that a step of fp32 is worth a power of two or more: the
+                    // first reference is the largest of them, which is exact, no weight is
+                    // more than its scale, and the other groups share that reference.
+                    const float own = fabsf(fmaxf(s[nt][j], s[nt][2 + j]));
+                    const bool far = __ballot_sync(0xffffffffu, own >= kKv4Far && own < INFINITY) & column;
                     const float r0 = st.r[nt][j];
                     float by0 = 0.f;
 #pragma unroll
                     for (int x = 0; x < NG; ++x) {
                         float top = -INFINITY;  // log2 of the largest weight as it is
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            top = fmaxf(top, fmaf(s[nt][2 * i + j], q.unit[nt][j], -r0) +
-                                                 fmaxf(fast_log2(va[i][x]), kKv4Least));
-                        if (x) top += fast_log2(st.f[x][nt][j]);
+                        for (int i = 0; i < 2; ++i) {
+                            const float at = s[nt][2 * i + j];
+                            top = fmaxf(top, far ? at : at - r0 + fmaxf(fast_log2(va[i][x]), kKv4Least));
+                        }
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1)
                             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const float lead = x ? fast_log2(st.f[x][nt][j]) : 0.f;
                         // up only, but from no reference to any
-                        float by = rintf(top - kKv4Shift);
-                        if (!move || !(by > (st.fresh ? -INFINITY : 0.f))) by = 0.f;
+                        float by = rintf(top + lead - kKv4Shift);
+                        if (far) by = x ? by0 + lead : top - r0;
+                        const bool up = move && by > (st.fresh ? -INFINITY : 0.f);
+                        if (!up) by = 0.f;
                         // without a reference the sums are 0
                         const float u = st.fresh ? 1.f : fast_exp2(-by);
 #pragma unroll
@@ -428,10 +436,12 @@ struct Kv4Block {
                         if constexpr (ADDED) z[x][nt][j] *= u;
                         if (x == 0) {
                             by0 = by;
-                            st.r[nt][j] = r0 + by;
+                            st.r[nt][j] = far && up ? top : r0 + by;
                             st.l[nt][j] *= u;
 #pragma unroll
                             for (int y = 0; y < NG; ++y) st.mid[y][nt][j] *= u;
+                        } else if (far && up) {
+                            st.f[x][nt][j] = 1.f;
                         } else {
                             st.f[x][nt][j] *= fast_exp2(by0 - by);
                         }
@@ -616,13 +626,13 @@ struct Kv4Format {
             // The next block's scores beside the products of the one before it.
             Kv4Block<D, NT> b[2];
             b[0].template score<false>(at, 0, 16, q, lane);
-            b[0].template weigh<false>(q, st, z, lane);
+            b[0].template weigh<false>(st, z, lane);
 #pragma unroll
             for (int i = 1; i < MT; ++i) {
                 b[i % 2].template score<false>(at, i, 16, q, lane);
                 if (i == 1) b[0].template apply<true>(at, 0, st, z);
                 else b[(i - 1) % 2].template apply<false>(at, i - 1, st, z);
-                b[i % 2].template weigh<true>(q, st, z, lane);
+                b[i % 2].template weigh<true>(st, z, lane);
             }
             b[(MT - 1) % 2].template apply<MT == 1>(at, MT - 1, st, z);
             st.centre(z);
@@ -631,7 +641,7 @@ struct Kv4Format {
             for (int i = 0; i * 16 < valid; ++i) {
                 Kv4Block<D, NT> b;
                 b.template score<true>(at, i, valid - i * 16, q, lane);
-                b.template weigh<false>(q, st, z, lane);
+                b.template weigh<false>(st, z, lane);
                 b.template apply<true>(at, i, st, z);
                 st.centre(z);
             }
