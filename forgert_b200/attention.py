@@ -339,8 +339,8 @@ class KV4Cache:
     codes to a byte, contiguous in the last dimension and both of the same
     strides, else of any; scales [num_pages, num_kv_heads, page_size, 2,
     head_dim / 64, 2] fp16, contiguous (for each row of K and of V the scale and
-    bias of each 64 dims).  The cache is the caller's memory: this keeps the
-    tensors and their layout.
+    bias of each 64 dims).  Codes of K, of V and scales below 64 GB each.  The
+    cache is the caller's memory: this keeps the tensors and their layout.
     """
 
     def __init__(self, k, v, scales):

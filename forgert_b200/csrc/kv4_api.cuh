@@ -18,8 +18,8 @@ int check_kv4(const fr_kv4_cache* c) {
     // scales below 64 GB each.
     const long long limit = 1LL << 32, pages = c->num_pages;
     const long long scales = (long long)c->num_kv_heads * c->page_size * (c->head_dim / 8) / 16;
-    if (c->page_stride >= limit || c->head_stride >= limit * 16 / c->num_kv_heads ||
-        c->row_stride >= limit * 16 / c->page_size || scales >= limit / pages ||
+    if (c->page_stride >= limit || c->head_stride > (limit * 16 - 1) / c->num_kv_heads ||
+        c->row_stride > (limit * 16 - 1) / c->page_size || scales > (limit - 1) / pages ||
         pages * (c->page_stride / 16) + c->num_kv_heads * (c->head_stride / 16) +
                 c->page_size * (c->row_stride / 16) >= limit)
         return FR_ERR_INVALID_ARG;
@@ -346,7 +346,8 @@ int fr_decode_attn_paged_kv4(const void* q, long long q_stride, const fr_kv4_cac
 
 size_t fr_kv4_workspace_size(int batch, int num_heads, int num_kv_heads, int head_dim,
                              int max_kv_len) {
-    if (batch <= 0 || max_kv_len < 0 || check_heads(num_heads, num_kv_heads, head_dim) != FR_OK)
+    if (batch <= 0 || max_kv_len < 0 || max_kv_len >= (1 << 30) ||
+        check_heads(num_heads, num_kv_heads, head_dim) != FR_OK)
         return 0;
     size_t bytes = 0;
     guarded([&]() -> int {

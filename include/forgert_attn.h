@@ -419,11 +419,13 @@ FR_API int fr_qkv_rope_append_paged(const void* q, const void* k, const void* v,
  * codes 0 .. 15, two to a byte (dim 2i in the low half of byte i, dim 2i + 1 in
  * the high half).  k and v hold the codes of
  * [num_pages][num_kv_heads][page_size][head_dim / 2 bytes]; the last dimension
- * is contiguous, the others have the strides given (in bytes, multiples of 16;
- * a page's below 2^32, a row's below 2^28).
+ * is contiguous, the others have the strides given (in bytes, multiples of 16).
  *   scales [num_pages][num_kv_heads][page_size][2 (K, V)][head_dim / FR_KV4_GROUP]
  *          [2 (scale, bias)] fp16, finite, scales not negative
- * Slot s is row s % page_size of page s / page_size. */
+ * Slot s is row s % page_size of page s / page_size.  Larger caches than these are
+ * refused (FR_ERR_INVALID_ARG): page_stride below 2^32; num_pages * page_stride +
+ * num_kv_heads * head_stride + page_size * row_stride below 2^36, and so the codes
+ * of K (or V) below 64 GB; the scales below 64 GB. */
 #define FR_KV4_GROUP 64
 
 typedef struct fr_kv4_cache {
