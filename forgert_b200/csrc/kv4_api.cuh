@@ -145,12 +145,20 @@ int run_kv4(const void* q, long long q_stride, const fr_kv4_cache* cache, const 
     p.max_units = kCachedUnits;
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(st->ws) + kCounterBytes);
     p.part_acc = p.part_ml + (size_t)2 * pl.ctas * 8 * pl.nt * 2;
-    // One tile per CTA is enough before SMs get more than one (two: 17 sequences of
-    // up to 2999 tokens, 12 / 2 heads of 128, 14.0 us instead of 11.8, no call
-    // measured faster).  A unit's start and its merge are charged as one tile each
-    // (none: 64 sequences of 1024 to 8192 45.5 -> 47.4, one of 512 7.4 -> 6.8; two:
-    // 46.4 and 8.0), and units of up to four tiles are not cut (one of 512 7.4 ->
-    // 7.1, 64 of 200 to 300 15.7 -> 9.9; six: one of 640 8.8 -> 10.1).
+    // The rules below were measured on 64 calls (28 / 4 and 16 / 1 heads of 128, 14 / 2
+    // and 8 / 8 of 64; 1 to 128 sequences of up to 8192 tokens).
+    // One tile per CTA is enough before SMs get more than one: with two no call is
+    // faster, and those of one to two tiles per SM leave half the copies that could
+    // be under way (24 sequences of 500 to 2000 tokens, 14 / 2 and 16 / 1 heads, 10.6
+    // and 11.9 -> 12.8 and 14.7 us; 64 of up to 1000, 14 / 2, 10.9 -> 13.3).
+    // A unit's start and its merge are charged as one tile each: without, one sequence
+    // gains (of 900 tokens 9.2 -> 8.5) and ragged batches lose (64 of 1024 to 8192,
+    // 28 / 4, 14 / 2 and 16 / 1 heads, 51.2, 20.1 and 31.4 -> 52.9, 21.4 and 33.7); as
+    // two, one of 900 takes 9.9 and most batches longer (52.4, 21.4, 30.9).
+    // Units of up to four tiles are not cut, since handing a piece over and merging it
+    // take a CTA about as long as four tiles do: with two, 64 of 200 to 300 take 15.8
+    // us instead of 10.1 and one of 512 (14 / 2) 7.5 instead of 7.1; with six, one of
+    // 700 takes 11.3 instead of 9.2 and 9.0 instead of 7.6 (14 / 2).
     p.min_tiles_per_cta = 1;
     p.min_ctas = st->sm_count;
     p.item_cost = 1;
