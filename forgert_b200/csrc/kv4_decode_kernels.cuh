@@ -15,20 +15,27 @@
 // A weight p a' enters the product with V as two fp16, itself rounded and what the
 // rounding takes off, on a reference of its own group's, 2^8 up, so that one as
 // small as 2^-22 of the largest keeps its bits.  (One fp16 alone: 64 sequences of
-// 8192 to 32768 tokens in 147 us instead of 170, but the outputs off by 3.0e-4 of
+// 8192 to 32768 tokens in 147 us instead of 171, but the outputs off by 3.0e-4 of
 // their 2-norm instead of 2.1e-4, which is what their rounding takes.)  l and the
-// middles are on the first group's reference, in fp32 from unrounded p.
+// middles are on the first group's reference, in fp32 from unrounded p.  What is
+// left beside the outputs' rounding are the fp32 sums of the products: 0.3e-4 on
+// those sequences, 0.9e-4 over 131072 positions, where the outputs are small beside
+// their terms (o centred at every block: 0.65e-4, and 3 % more time).
 //
 // Bytes: D of codes per position and kv head, D / 8 of scales; 4 * D * G
-// operations on them.  Measured, 28 / 4 heads of 128: 64 sequences of 8192 to 32768
-// tokens (1.2 million tokens, 697 MB) 147 us, 4.7 TB/s, 0.72 of a copy's rate; of
-// 1024 to 8192 45 us; one sequence of 512 tokens 7.4 (14 / 2 heads of 64).  Bound by
-// the warps' instructions: the copies alone take 106 and 32 us.  At D = 128 a block
-// of 16 positions and one kv head takes a warp about 290, 124 of them on the integer
-// pipe, which takes one in two cycles: 80 masks and shifts of codes (5 for 8
-// codes), beside 18 products of 8 cycles each; 43 are a half of a step's overhead.
-// Twelve warps per SM issue in 55 to 59 % of the cycles whatever the order of the
-// phases (scores of two blocks at once, V loaded early or late: within 1 %).
+// operations on them.  Measured in graphs of 20 calls, 28 / 4 heads of 128: 64
+// sequences of 8192 to 32768 tokens (1.2 million tokens, 697 MB) 171 us, 4.1 TB/s,
+// 0.62 of a copy's rate; of 1024 to 8192 51 us; one sequence of 512 tokens 7.2 (14 /
+// 2 heads of 64).  The copies alone take 106 of the 171 and 32 of the 51 us.  No
+// pipe is full (issue slots 57 %, integer 43 %, tensor 36 %, fp32 23 %, DRAM 0.55 of
+// a copy's rate at 64 x 12288): what bounds it is the latency of a block's chain
+// (codes, scores, weights, transposed weights, products) at three warps a scheduler,
+// more of which the state leaves no registers for.  At D = 128 a block of 16
+// positions and one kv head takes a warp 335 instructions, 127 of them on the
+// integer pipe, which takes one in two cycles (80 masks and shifts of codes, 5 for 8
+// codes), and 28 products of 8 cycles each; 43 are a half of a step's overhead.  The
+// order of the phases changes little (scores of two blocks at once, V loaded early
+// or late: within 1 %, with weights in one fp16).
 //
 // Fragments (mma m16n8k16): of K a lane holds 16 dims of each group in rows 2g and
 // 2g + 1 of the block, as they lie in memory; contraction order is free, so q is

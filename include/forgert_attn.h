@@ -471,8 +471,9 @@ FR_API int fr_kv4_gather(const fr_kv4_cache* cache, const long long* slots, void
  * used, whatever they hold.  A NaN scale or bias of a used row makes the outputs
  * it enters NaN; outputs are 65504 at most.  Scores and sums are fp32, weights (a
  * probability times V's scale) keep 22 bits: a call is off by the rounding of its
- * outputs and hardly more, whatever max_kv_len.  The result does not depend on
- * which CTA merges: equal inputs give equal bits. */
+ * outputs and, where these are small beside the values they average, by fp32's
+ * rounding of the values' sums, whatever max_kv_len.  The result does not depend
+ * on which CTA merges: equal inputs give equal bits. */
 FR_API int fr_decode_attn_paged_kv4(const void* q, long long q_stride, const fr_kv4_cache* cache,
                                     const int* block_table, const int* kv_lens, void* out,
                                     int batch, int num_heads, int max_blocks_per_seq,
