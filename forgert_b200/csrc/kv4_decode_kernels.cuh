@@ -175,8 +175,8 @@ struct Kv4Query {
 };
 
 // Running state of a warp over an item, per head column.  r is the reference of
-// the first group's weights, in base 2 and a whole number, f[x] 2^(r - that of
-// group x).  o: products with V's codes from 7.5 on, in units of 2^-24 (even dims)
+// the first group's weights, in base 2 and a whole number (or a score, where these
+// are far from 0), f[x] 2^(r - that of group x).  o: products with V's codes from 7.5 on, in units of 2^-24 (even dims)
 // and 2^-28 (odd ones); mid: this lane's rows' part of sum p mid, l that of the row
 // sum, both on r.
 template <int D, int NT>
@@ -357,7 +357,7 @@ struct Kv4Block {
         }
     }
 
-    // Probabilities, their sums, and the weights P^T a' as fp16.  Where the weights
+    // Probabilities, their sums, and the weights P^T a' as two fp16.  Where the weights
     // of a column's rows here sum up to more than 2^15 or to NaN (in fp32, on a pipe
     // with room; with p as weights of the least scale among them), the column's
     // references move, by the scores and finite scales alone: p is finite then.
